@@ -25,7 +25,9 @@ ext = CUDAExtension(
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
-        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950"],
+        # no packed fp32 arithmetic: some of its forms have given wrong results
+        "nvcc": ["-O3", "-std=c++17", "--offload-arch=gfx950",
+                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
     },
 )
 
