@@ -23,6 +23,7 @@ from learning_at_home_amd.models import TransformerDMoE, TransformerDMoEConfig
 from learning_at_home_amd.parallel import ExpertParallelMoE, FusedExpertSGD
 from learning_at_home_amd.averaging import RcclAverager
 from learning_at_home_amd.ops import HAS_HIP
+from learning_at_home_amd.ops.functional import grad_clip_scale
 from learning_at_home_amd.optim import MasterSGD
 
 
@@ -36,7 +37,8 @@ def build_model(cfg: TransformerDMoEConfig, args, device, group=None):
         return ExpertParallelMoE(
             d_model=c.d_model, ffn_dim=c.ffn_dim, num_experts=c.num_experts,
             k=c.k_best, capacity_factor=args.capacity_factor,
-            aux_loss_coef=args.aux_coef, group=group, a2a_chunks=chunks,
+            aux_loss_coef=args.aux_coef, group=group,
+            a2a_chunks=1 if args.dropless else chunks, dropless=args.dropless,
         )
 
     model = TransformerDMoE(cfg, moe_factory)
@@ -98,6 +100,12 @@ def main():
     p.add_argument("--loss-every", type=int, default=0,
                    help="if >0, rank 0 prints the step loss to stderr every N "
                         "timed steps (long-horizon stability monitoring)")
+    p.add_argument("--dropless", action="store_true",
+                   help="experts without capacity: rows sorted by expert, ragged "
+                        "products, nothing dropped (default: capacity buffers)")
+    p.add_argument("--clip-norm", type=float, default=0.0,
+                   help="if >0, bound the norm of all gradients together (trunk and "
+                        "expert shards of this rank) to this; scaled on the GPU")
     p.add_argument("--no-dht", action="store_true",
                    help="skip the per-rank Kademlia DHT peer + expert announce "
                         "(north-star parity: each GPU rank hosts a shard AND a "
@@ -224,9 +232,14 @@ def main():
         trunk_opt.zero_grad(set_to_none=True)
         with tm("backward"):
             loss.backward()
+        scale = None
+        if args.clip_norm > 0 and use_cuda:
+            grads = trunk_opt.gradients() + [g for opt in expert_opts for g in opt.gradients()]
+            scale = grad_clip_scale(grads, args.clip_norm)[1]
+        scaled = {} if scale is None else {"grad_scale": scale}
         with tm("expert_opt"):
             for opt in expert_opts:
-                opt.step()  # async per-shard SGD (fused on GPU)
+                opt.step(**scaled)  # async per-shard SGD (fused on GPU)
                 if isinstance(opt, torch.optim.SGD):
                     opt.zero_grad(set_to_none=True)
         if averager is not None:
@@ -236,7 +249,7 @@ def main():
                 if isinstance(trunk_opt, MasterSGD):
                     trunk_opt.sync_masters_from_params()  # averaged values win
         with tm("trunk_opt"):
-            trunk_opt.step()
+            trunk_opt.step(**scaled)
         if averager is not None and (step_idx + 1) % args.averaging_period == 0:
             averager.step(async_op=True)  # overlapped on the side stream
             averager._round_pending = True
@@ -284,7 +297,9 @@ def main():
     drop_fracs = []
     for block in model.blocks:
         c = block.moe.last_counts
-        if c is not None:
+        if c is not None and args.dropless:
+            drop_fracs.append(0.0)
+        elif c is not None:
             cap = block.moe.capacity(tokens_per_step_per_rank)
             total = float(c.sum().item())
             kept = float(c.clamp(max=cap).sum().item())

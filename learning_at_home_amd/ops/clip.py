@@ -1,0 +1,117 @@
+"""Global gradient norm over many tensors, clipping, and the clipped SGD step.
+
+    norm, scale = grad_clip_scale(grads, max_norm)      # on the GPU, no host read
+    master_sgd_step_(params, masters, grads, lr=lr, grad_scale=scale)
+
+or, for an optimizer that knows nothing of it, clip_grad_norm_(grads, max_norm)
+in place. On a GPU a few launches serve all tensors (clip.hip); on the CPU, and
+for tensors the kernels do not take (not contiguous), plain torch.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _C, HAS_HIP
+
+_KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _listed(tensors) -> list:
+    if isinstance(tensors, torch.Tensor):
+        tensors = [tensors]
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError("no tensors")
+    if any(t.device != tensors[0].device for t in tensors):
+        raise ValueError("all tensors must be on one device")
+    return tensors
+
+
+def _kernels_take(tensors) -> bool:
+    return (HAS_HIP and tensors[0].is_cuda
+            and all(t.dtype in _KERNEL_TYPES and t.is_contiguous() for t in tensors))
+
+
+@torch.no_grad()
+def grad_clip_scale(tensors: Sequence[torch.Tensor], max_norm: float,
+                    eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(norm, scale), two fp32 numbers on the tensors' device: the 2-norm of all
+    tensors together, and min(1, max_norm / (norm + eps)). A gradient that is
+    not finite makes a norm that is not (scale 0 for infinity, not-a-number for
+    one). The norm is this process's own: steps here wait for no other rank."""
+    tensors = _listed(tensors)
+    if not max_norm > 0:
+        raise ValueError(f"max_norm must be positive, got {max_norm}")
+    if tensors[0].is_cuda and HAS_HIP:
+        tensors = [t.contiguous() for t in tensors]
+        if _kernels_take(tensors):
+            return tuple(_C.grad_norm(tensors, max_norm, eps))
+    norm = torch.stack([t.float().square().sum(dtype=torch.float64) for t in tensors]).sum().sqrt()
+    return norm.float(), (max_norm / (norm + eps)).clamp(max=1.0).float()
+
+
+@torch.no_grad()
+def clip_grad_norm_(tensors: Sequence[torch.Tensor], max_norm: float,
+                    eps: float = 1e-6) -> torch.Tensor:
+    """Scales the tensors in place to a common 2-norm of at most max_norm, and
+    returns the norm they had, on their device."""
+    tensors = _listed(tensors)
+    norm, scale = grad_clip_scale(tensors, max_norm, eps)
+    if _kernels_take(tensors):
+        _C.grad_scale_(tensors, scale)
+    else:
+        for t in tensors:
+            t.mul_(scale.to(t.dtype) if t.dtype == torch.float64 else scale)
+    return norm
+
+
+@torch.no_grad()
+def master_sgd_step_(params: Sequence[torch.Tensor], masters: Sequence[torch.Tensor],
+                     grads: Sequence[torch.Tensor], lr: float, momentum: float = 0.0,
+                     weight_decay: float = 0.0,
+                     momentum_bufs: Optional[Sequence[torch.Tensor]] = None,
+                     grad_scale: Optional[torch.Tensor] = None) -> None:
+    """One SGD step of fp32 masters, all tensors at once:
+
+        u = grad_scale * g + weight_decay * m
+        b = momentum * b + u, u = b          (with momentum_bufs)
+        m -= lr * u;  p = m rounded to p's type
+    """
+    params, masters, grads = list(params), list(masters), list(grads)
+    bufs = list(momentum_bufs) if momentum_bufs is not None else []
+    if not len(params) == len(masters) == len(grads) or (bufs and len(bufs) != len(params)):
+        raise ValueError("params, masters, grads and momentum_bufs must go together")
+    if momentum and not bufs:
+        raise ValueError("momentum needs momentum_bufs")
+    if any(p.shape != m.shape or p.shape != g.shape for p, m, g in zip(params, masters, grads)):
+        raise ValueError("params, masters and grads must have the same shapes")
+    if any(p.shape != b.shape for p, b in zip(params, bufs)):
+        raise ValueError("momentum_bufs must have the shapes of the params")
+    if any(m.dtype != torch.float32 for m in masters + bufs):
+        raise ValueError("masters and momentum_bufs must be fp32")
+    if not params:
+        return
+    fits = [HAS_HIP and p.is_cuda and p.dtype == torch.bfloat16 and g.dtype in _KERNEL_TYPES
+            and p.is_contiguous() and m.is_contiguous() and g.is_contiguous()
+            for p, m, g in zip(params, masters, grads)]
+    if bufs:
+        fits = [f and b.is_contiguous() for f, b in zip(fits, bufs)]
+    if all(fits):
+        _C.master_sgd_(params, masters, grads, bufs, grad_scale, lr, momentum, weight_decay)
+        return
+    some = [i for i, f in enumerate(fits) if f]
+    if some:
+        _C.master_sgd_(*([t[i] for i in some] for t in (params, masters, grads)),
+                       [bufs[i] for i in some] if bufs else [], grad_scale, lr, momentum, weight_decay)
+    for i in (i for i, f in enumerate(fits) if not f):
+        u = grads[i].float()
+        if grad_scale is not None:
+            u = u * grad_scale
+        if weight_decay:
+            u = u + weight_decay * masters[i]
+        if bufs:
+            u = bufs[i].mul_(momentum).add_(u)
+        masters[i].add_(u, alpha=-lr)
+        params[i].copy_(masters[i])

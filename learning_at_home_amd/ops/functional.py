@@ -371,3 +371,11 @@ def expert_ffn_reference(x, W1, b1, W2, b2):
     """fp32 reference of one expert FFN: gelu_tanh(x@W1^T+b1)@W2^T+b2."""
     h = F.gelu(x.float() @ W1.float().t() + b1.float(), approximate="tanh")
     return h @ W2.float().t() + b2.float()
+
+
+# experts without capacity, and gradient clipping (files of their own)
+from .clip import clip_grad_norm_, grad_clip_scale, master_sgd_step_  # noqa: E402, F401
+from .ragged import (  # noqa: E402, F401
+    RaggedLayout, grouped_linear, ragged_combine, ragged_ffn, ragged_gather, ragged_layout,
+    ragged_ungather,
+)

@@ -30,17 +30,31 @@ void lah_combine_bwd(const void*, const void*, const void*, const void*, const v
                      const void*, void*, void*, int, int, int, int, hipStream_t);
 void lah_zero_padding(const void*, void*, int, int, int, hipStream_t);
 void lah_sgd_step(void*, const void*, void*, void*, long, float, float, float,
-                  hipStream_t);
+                  const void*, hipStream_t);
 void lah_sgd_step_t(void*, const void*, void*, void*, int, int, int, float, float,
-                    hipStream_t);
+                    const void*, hipStream_t);
 void lah_sgd_step_sr_t(void*, const void*, void*, int, int, int, float, float,
-                       unsigned, hipStream_t);
+                       unsigned, const void*, hipStream_t);
 void lah_transpose_bf16(const void*, void*, int, int, int, hipStream_t);
 void lah_ce_rowstats(const void*, const void*, void*, void*, int, long, int, int,
                      hipStream_t);
 void lah_ce_bwd(const void*, const void*, const void*, void*, float, int, long, int,
                 int, hipStream_t);
 void lah_colsum(const void*, void*, int, int, int, hipStream_t);
+long lah_ragged_layout_table(long, int);
+void lah_ragged_layout(const void*, int, long, int, void*, void*, void*, void*, hipStream_t);
+void lah_ragged_nt(const void*, const void*, void*, const void*, const void*, int, void*,
+                   long, int, int, int, int, hipStream_t);
+void lah_ragged_nn(const void*, const void*, void*, const void*, void*, long, int, int, int,
+                   hipStream_t);
+void lah_ragged_tn(const void*, const void*, void*, void*, int, const void*, long, int, int,
+                   int, int, hipStream_t);
+long lah_clip_partials(int);
+void lah_grad_norm(void* const*, const long*, const int*, int, void*, float, float, void*,
+                   void*, hipStream_t);
+void lah_grad_scale(void* const*, const long*, const int*, int, const void*, hipStream_t);
+void lah_master_sgd(void* const*, void* const*, void* const*, void* const*, const long*,
+                    const int*, int, const void*, float, float, float, hipStream_t);
 }
 
 namespace {
@@ -235,8 +249,18 @@ std::vector<torch::Tensor> combine_bwd(torch::Tensor dy, torch::Tensor ybuf,
   return {dybuf, dw};
 }
 
+// the clipping factor, one fp32 number on the GPU, or null
+const void* scale_ptr(const c10::optional<torch::Tensor>& s, const torch::Tensor& like) {
+  if (!s.has_value()) return nullptr;
+  CHECK_F32(*s);
+  TORCH_CHECK(s->numel() == 1 && s->device() == like.device(),
+              "the gradients' scale must be one number on their GPU");
+  return s->data_ptr();
+}
+
 void sgd_step(torch::Tensor master, torch::Tensor grad, c10::optional<torch::Tensor> momentum,
-              torch::Tensor out_bf16, double lr, double mu, double weight_decay) {
+              torch::Tensor out_bf16, double lr, double mu, double weight_decay,
+              c10::optional<torch::Tensor> gscale) {
   CHECK_F32(master); CHECK_F32(grad); CHECK_BF16(out_bf16);
   CHECK_CONTIG(master); CHECK_CONTIG(grad); CHECK_CONTIG(out_bf16);
   long n = master.numel();
@@ -245,28 +269,32 @@ void sgd_step(torch::Tensor master, torch::Tensor grad, c10::optional<torch::Ten
   void* mom_p = nullptr;
   if (momentum.has_value()) { CHECK_F32(*momentum); mom_p = momentum->data_ptr(); }
   lah_sgd_step(master.data_ptr(), grad.data_ptr(), mom_p, out_bf16.data_ptr(), n, (float)lr,
-               (float)mu, (float)weight_decay, cur_stream());
+               (float)mu, (float)weight_decay, scale_ptr(gscale, master), cur_stream());
 }
 
 void sgd_step_t(torch::Tensor master, torch::Tensor grad, torch::Tensor out,
-                torch::Tensor outT, double lr, double weight_decay) {
+                torch::Tensor outT, double lr, double weight_decay,
+                c10::optional<torch::Tensor> gscale) {
   CHECK_F32(master); CHECK_F32(grad); CHECK_BF16(out); CHECK_BF16(outT);
   CHECK_CONTIG(master); CHECK_CONTIG(grad); CHECK_CONTIG(out); CHECK_CONTIG(outT);
   int E = master.size(0), R = master.size(1), C = master.size(2);
   TORCH_CHECK(R % 64 == 0 && C % 64 == 0, "dims must be multiples of 64");
   TORCH_CHECK(outT.size(1) == C && outT.size(2) == R, "outT must be [E, C, R]");
   lah_sgd_step_t(master.data_ptr(), grad.data_ptr(), out.data_ptr(), outT.data_ptr(),
-                 E, R, C, (float)lr, (float)weight_decay, cur_stream());
+                 E, R, C, (float)lr, (float)weight_decay, scale_ptr(gscale, master),
+                 cur_stream());
 }
 
 void sgd_step_sr_t(torch::Tensor param, torch::Tensor grad, torch::Tensor paramT,
-                   double lr, double weight_decay, int64_t seed) {
+                   double lr, double weight_decay, int64_t seed,
+                   c10::optional<torch::Tensor> gscale) {
   CHECK_BF16(param); CHECK_F32(grad); CHECK_BF16(paramT);
   CHECK_CONTIG(param); CHECK_CONTIG(grad); CHECK_CONTIG(paramT);
   int E = param.size(0), R = param.size(1), C = param.size(2);
   TORCH_CHECK(R % 64 == 0 && C % 64 == 0, "dims must be multiples of 64");
   lah_sgd_step_sr_t(param.data_ptr(), grad.data_ptr(), paramT.data_ptr(), E, R, C,
-                    (float)lr, (float)weight_decay, (unsigned)seed, cur_stream());
+                    (float)lr, (float)weight_decay, (unsigned)seed,
+                    scale_ptr(gscale, param), cur_stream());
 }
 
 torch::Tensor transpose_bf16(torch::Tensor in) {
@@ -342,6 +370,218 @@ std::vector<torch::Tensor> flash_attn_bwd(torch::Tensor q, torch::Tensor k,
   return {dq, dk, dv};
 }
 
+// ---- products grouped by expert, ragged sizes (ragged_gemm.hip, ragged_layout.hip) ----
+
+// Work goes to the tensors' own device, on its current stream.
+#define ON_DEVICE_OF(t) const c10::OptionalDeviceGuard device_guard(at::device_of(t))
+#define CHECK_LAUNCH()                                                      \
+  do {                                                                      \
+    const hipError_t err = hipGetLastError();                               \
+    TORCH_CHECK(err == hipSuccess, "launch: ", hipGetErrorString(err));     \
+  } while (0)
+#define CHECK_ALIGNED(t) \
+  TORCH_CHECK(((uintptr_t)(t).data_ptr() & 15) == 0, #t " must start at a multiple of 16 bytes")
+
+static void check_ragged(const torch::Tensor& a, const torch::Tensor& b,
+                         const torch::Tensor& offsets) {
+  for (const auto* t : {&a, &b}) {
+    CHECK_CUDA(*t); CHECK_BF16(*t); CHECK_CONTIG(*t); CHECK_ALIGNED(*t);
+  }
+  CHECK_I32(offsets); CHECK_CONTIG(offsets);
+  TORCH_CHECK(offsets.dim() == 1 && offsets.numel() >= 2, "offsets must be [E + 1], E >= 1");
+  TORCH_CHECK(a.device() == b.device() && a.device() == offsets.device(),
+              "all tensors must be on one GPU");
+  TORCH_CHECK(a.dim() == 2 && a.size(0) < (int64_t)1 << 31, "rows must be [R, K], R < 2^31");
+}
+
+static void check_weight(const torch::Tensor& w, const torch::Tensor& offsets) {
+  TORCH_CHECK(w.dim() == 3 && w.size(0) == offsets.numel() - 1, "weight must be [E, N, K]");
+  TORCH_CHECK(w.size(1) > 0 && w.size(2) > 0 && w.size(1) % 8 == 0 && w.size(2) % 8 == 0,
+              "N and K must be multiples of 8");
+  TORCH_CHECK(w.size(1) * w.size(2) < (int64_t)1 << 30, "N * K must be below 2^30");
+}
+
+std::vector<torch::Tensor> ragged_layout(torch::Tensor ids, int64_t E) {
+  CHECK_CUDA(ids); CHECK_CONTIG(ids);
+  const bool wide = ids.scalar_type() == at::kLong;
+  TORCH_CHECK(wide || ids.scalar_type() == at::kInt, "ids must be int32 or int64");
+  TORCH_CHECK(E >= 1 && E <= 4096, "1 to 4096 experts, got ", E);
+  const int64_t n = ids.numel();
+  TORCH_CHECK(n < ((int64_t)1 << 31) - 65536, "too many slots");
+  ON_DEVICE_OF(ids);
+  const auto opt = ids.options().dtype(at::kInt);
+  auto offsets = torch::empty({E + 1}, opt), order = torch::empty({n}, opt);
+  auto rows = torch::empty(ids.sizes(), opt);
+  torch::Tensor table;
+  if (const long room = lah_ragged_layout_table(n, (int)E)) table = torch::empty({room}, opt);
+  lah_ragged_layout(ids.data_ptr(), wide, n, (int)E, table.defined() ? table.data_ptr() : nullptr,
+                    offsets.data_ptr(), order.data_ptr(), rows.data_ptr(), cur_stream());
+  CHECK_LAUNCH();
+  return {offsets, order, rows};
+}
+
+// y[r] = act(W[e] x[r] + b[e]); epi 0 plain, 1 gelu, 2 gelu and its slope into der
+torch::Tensor ragged_nt(torch::Tensor x, torch::Tensor w, torch::Tensor offsets,
+                        c10::optional<torch::Tensor> bias, c10::optional<torch::Tensor> der,
+                        int64_t epi) {
+  check_ragged(x, w, offsets);
+  check_weight(w, offsets);
+  const int64_t R = x.size(0), E = w.size(0), N = w.size(1), K = w.size(2);
+  TORCH_CHECK(x.size(1) == K, "x must be [R, ", K, "], got [", R, ", ", x.size(1), "]");
+  TORCH_CHECK(epi >= 0 && epi <= 2 && (epi == 2) == der.has_value(), "epi 2 goes with der");
+  const void* bias_p = nullptr;
+  int bias_bf16 = 0;
+  if (bias.has_value()) {
+    CHECK_CONTIG(*bias); CHECK_ALIGNED(*bias);
+    bias_bf16 = bias->scalar_type() == at::kBFloat16;
+    TORCH_CHECK(bias_bf16 || bias->scalar_type() == at::kFloat, "bias must be bf16 or fp32");
+    TORCH_CHECK(bias->dim() == 2 && bias->size(0) == E && bias->size(1) == N &&
+                bias->device() == x.device(), "bias must be [E, N] on the GPU of x");
+    bias_p = bias->data_ptr();
+  }
+  void* der_p = nullptr;
+  if (der.has_value()) {
+    CHECK_BF16(*der); CHECK_CONTIG(*der); CHECK_ALIGNED(*der);
+    TORCH_CHECK(der->dim() == 2 && der->size(0) == R && der->size(1) == N &&
+                der->device() == x.device(), "der must be [R, N] on the GPU of x");
+    der_p = der->data_ptr();
+  }
+  ON_DEVICE_OF(x);
+  auto y = torch::empty({R, N}, x.options());
+  if (R == 0) return y;
+  lah_ragged_nt(x.data_ptr(), w.data_ptr(), y.data_ptr(), offsets.data_ptr(), bias_p, bias_bf16,
+                der_p, R, (int)E, (int)N, (int)K, (int)epi, cur_stream());
+  CHECK_LAUNCH();
+  return y;
+}
+
+// out[r] = W[e]^T d[r], times der[r] if given
+torch::Tensor ragged_nn(torch::Tensor d, torch::Tensor w, torch::Tensor offsets,
+                        c10::optional<torch::Tensor> der) {
+  check_ragged(d, w, offsets);
+  check_weight(w, offsets);
+  const int64_t R = d.size(0), E = w.size(0), K = w.size(1), N = w.size(2);
+  TORCH_CHECK(d.size(1) == K, "d must be [R, ", K, "], got [", R, ", ", d.size(1), "]");
+  void* der_p = nullptr;
+  if (der.has_value()) {
+    CHECK_BF16(*der); CHECK_CONTIG(*der); CHECK_ALIGNED(*der);
+    TORCH_CHECK(der->dim() == 2 && der->size(0) == R && der->size(1) == N &&
+                der->device() == d.device(), "der must be [R, N] on the GPU of d");
+    der_p = der->data_ptr();
+  }
+  ON_DEVICE_OF(d);
+  auto out = torch::empty({R, N}, d.options());
+  if (R == 0) return out;
+  lah_ragged_nn(d.data_ptr(), w.data_ptr(), out.data_ptr(), offsets.data_ptr(), der_p, R, (int)E,
+                (int)N, (int)K, cur_stream());
+  CHECK_LAUNCH();
+  return out;
+}
+
+// dw[e] = sum_r d[r] x[r]^T (added to what is there if accumulate), db[e] = sum_r d[r]
+void ragged_tn(torch::Tensor d, torch::Tensor x, torch::Tensor offsets, torch::Tensor dw,
+               c10::optional<torch::Tensor> db, bool accumulate) {
+  check_ragged(d, x, offsets);
+  const int64_t R = d.size(0), M = d.size(1), E = offsets.numel() - 1;
+  TORCH_CHECK(x.dim() == 2 && x.size(0) == R, "d and x must have the same rows");
+  const int64_t N = x.size(1);
+  CHECK_CONTIG(dw); CHECK_ALIGNED(dw);
+  const bool bf16 = dw.scalar_type() == at::kBFloat16;
+  TORCH_CHECK(bf16 || dw.scalar_type() == at::kFloat, "dw must be bf16 or fp32");
+  TORCH_CHECK(!(bf16 && accumulate), "sums over several calls are held in fp32");
+  TORCH_CHECK(dw.dim() == 3 && dw.size(1) == M && dw.size(2) == N && dw.device() == d.device(),
+              "dw must be [E, M, N] on the GPU of d");
+  check_weight(dw, offsets);
+  void* db_p = nullptr;
+  int db_bf16 = 0;
+  if (db.has_value()) {
+    CHECK_CONTIG(*db);
+    db_bf16 = db->scalar_type() == at::kBFloat16;
+    TORCH_CHECK(db_bf16 || db->scalar_type() == at::kFloat, "db must be bf16 or fp32");
+    TORCH_CHECK(!(db_bf16 && accumulate), "sums over several calls are held in fp32");
+    TORCH_CHECK(db->dim() == 2 && db->size(0) == E && db->size(1) == M &&
+                db->device() == d.device(), "db must be [E, M] on the GPU of d");
+    db_p = db->data_ptr();
+  }
+  ON_DEVICE_OF(d);
+  lah_ragged_tn(d.data_ptr(), x.data_ptr(), dw.data_ptr(), db_p, db_bf16, offsets.data_ptr(), R,
+                (int)E, (int)N, (int)M, bf16 ? 2 : accumulate ? 1 : 0, cur_stream());
+  CHECK_LAUNCH();
+}
+
+// ---- gradient norm, clipping, clipped step of fp32 masters (clip.hip) ----
+
+static int clip_kind(const torch::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return 0;
+    case at::kHalf: return 1;
+    case at::kFloat: return 2;
+    default: TORCH_CHECK(false, "gradients must be bf16, fp16 or fp32, got ", t.scalar_type());
+  }
+}
+
+struct ClipList {
+  std::vector<void*> p;
+  std::vector<long> n;
+  std::vector<int> kind;
+  explicit ClipList(const std::vector<torch::Tensor>& ts) {
+    TORCH_CHECK(!ts.empty(), "no tensors");
+    for (const auto& t : ts) {
+      CHECK_CUDA(t);
+      TORCH_CHECK(t.device() == ts[0].device(), "all tensors must be on one GPU");
+      CHECK_CONTIG(t);
+      p.push_back(t.data_ptr());
+      n.push_back(t.numel());
+      kind.push_back(clip_kind(t));
+    }
+  }
+};
+
+std::vector<torch::Tensor> grad_norm(std::vector<torch::Tensor> grads, double max_norm, double eps) {
+  const ClipList l(grads);
+  ON_DEVICE_OF(grads[0]);
+  const auto opt = grads[0].options();
+  auto partial = torch::empty({lah_clip_partials((int)l.p.size())}, opt.dtype(at::kDouble));
+  auto norm = torch::empty({}, opt.dtype(at::kFloat)), scale = torch::empty({}, opt.dtype(at::kFloat));
+  lah_grad_norm(l.p.data(), l.n.data(), l.kind.data(), (int)l.p.size(), partial.data_ptr(),
+                (float)max_norm, (float)eps, norm.data_ptr(), scale.data_ptr(), cur_stream());
+  CHECK_LAUNCH();
+  return {norm, scale};
+}
+
+void grad_scale_(std::vector<torch::Tensor> grads, torch::Tensor scale) {
+  const ClipList l(grads);
+  const void* s = scale_ptr(scale, grads[0]);
+  ON_DEVICE_OF(grads[0]);
+  lah_grad_scale(l.p.data(), l.n.data(), l.kind.data(), (int)l.p.size(), s, cur_stream());
+  CHECK_LAUNCH();
+}
+
+void master_sgd_(std::vector<torch::Tensor> params, std::vector<torch::Tensor> masters,
+                 std::vector<torch::Tensor> grads, std::vector<torch::Tensor> bufs,
+                 c10::optional<torch::Tensor> scale, double lr, double mu, double weight_decay) {
+  const ClipList p(params), m(masters), g(grads);
+  TORCH_CHECK(p.n == m.n && p.n == g.n, "params, masters and grads must have the same sizes");
+  TORCH_CHECK(params[0].device() == masters[0].device() && params[0].device() == grads[0].device(),
+              "all tensors must be on one GPU");
+  std::vector<void*> b;
+  if (!bufs.empty()) {
+    const ClipList l(bufs);
+    TORCH_CHECK(l.n == p.n && bufs[0].device() == params[0].device(),
+                "momentum buffers must have the sizes of the params");
+    for (const int k : l.kind) TORCH_CHECK(k == 2, "momentum buffers must be fp32");
+    b = l.p;
+  }
+  for (const int k : p.kind) TORCH_CHECK(k == 0, "params must be bf16");
+  for (const int k : m.kind) TORCH_CHECK(k == 2, "masters must be fp32");
+  const void* s = scale_ptr(scale, params[0]);
+  ON_DEVICE_OF(params[0]);
+  lah_master_sgd(p.p.data(), m.p.data(), g.p.data(), b.empty() ? nullptr : b.data(), p.n.data(),
+                 g.kind.data(), (int)p.p.size(), s, (float)lr, (float)mu, (float)weight_decay,
+                 cur_stream());
+  CHECK_LAUNCH();
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("batched_gemm_nt", &batched_gemm_nt, "batched NT GEMM with fused epilogue",
         py::arg("A"), py::arg("B"), py::arg("bias") = py::none(),
@@ -368,12 +608,25 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("combine_bwd", &combine_bwd);
   m.def("sgd_step", &sgd_step, py::arg("master"), py::arg("grad"),
         py::arg("momentum"), py::arg("out_bf16"),
-        py::arg("lr") = 0.01, py::arg("mu") = 0.0, py::arg("weight_decay") = 0.0);
+        py::arg("lr") = 0.01, py::arg("mu") = 0.0, py::arg("weight_decay") = 0.0,
+        py::arg("gscale") = py::none());
   m.def("sgd_step_t", &sgd_step_t, py::arg("master"), py::arg("grad"), py::arg("out"),
-        py::arg("outT"), py::arg("lr") = 0.01, py::arg("weight_decay") = 0.0);
+        py::arg("outT"), py::arg("lr") = 0.01, py::arg("weight_decay") = 0.0,
+        py::arg("gscale") = py::none());
   m.def("sgd_step_sr_t", &sgd_step_sr_t, py::arg("param"), py::arg("grad"),
         py::arg("paramT"), py::arg("lr") = 0.01, py::arg("weight_decay") = 0.0,
-        py::arg("seed") = 0);
+        py::arg("seed") = 0, py::arg("gscale") = py::none());
   m.def("transpose_bf16", &transpose_bf16);
   m.def("colsum", &colsum);
+  m.def("ragged_layout", &ragged_layout, py::arg("ids"), py::arg("num_experts"));
+  m.def("ragged_nt", &ragged_nt, py::arg("x"), py::arg("w"), py::arg("offsets"),
+        py::arg("bias") = py::none(), py::arg("der") = py::none(), py::arg("epi") = 0);
+  m.def("ragged_nn", &ragged_nn, py::arg("d"), py::arg("w"), py::arg("offsets"),
+        py::arg("der") = py::none());
+  m.def("ragged_tn", &ragged_tn, py::arg("d"), py::arg("x"), py::arg("offsets"), py::arg("dw"),
+        py::arg("db") = py::none(), py::arg("accumulate") = false);
+  m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("max_norm"), py::arg("eps") = 1e-6);
+  m.def("grad_scale_", &grad_scale_, py::arg("grads"), py::arg("scale"));
+  m.def("master_sgd_", &master_sgd_, py::arg("params"), py::arg("masters"), py::arg("grads"),
+        py::arg("bufs"), py::arg("scale"), py::arg("lr"), py::arg("mu"), py::arg("weight_decay"));
 }

@@ -9,10 +9,21 @@
 
 typedef __attribute__((ext_vector_type(4))) float f4;
 
+// SCALED (all three step kernels): the gradient times *gscale, the clipping
+// factor that clip.hip leaves on the GPU, so a clipped step writes no gradients.
+// The product is rounded by itself: a scaled step is the step of the scaled
+// gradient, bit for bit.
+LAH_DEVINL float scaled_grad(float g, float s) {
+#pragma clang fp contract(off)
+  return g * s;
+}
+
+template <bool SCALED>
 __global__ void sgd_step_kernel(float* __restrict__ master, const float* __restrict__ grad,
                                 float* __restrict__ momentum,  // null = plain SGD
                                 __bf16* __restrict__ out_bf16, long n, float lr,
-                                float mu, float weight_decay) {
+                                float mu, float weight_decay, const float* __restrict__ gscale) {
+  const float gs = SCALED ? *gscale : 1.0f;
   long i = ((long)blockIdx.x * blockDim.x + threadIdx.x) * 4;
   long stride = (long)gridDim.x * blockDim.x * 4;
   for (; i + 3 < n; i += stride) {
@@ -20,7 +31,7 @@ __global__ void sgd_step_kernel(float* __restrict__ master, const float* __restr
     f4 g = *(const f4*)(grad + i);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      float gq = g[q] + weight_decay * m[q];
+      float gq = (SCALED ? scaled_grad(g[q], gs) : g[q]) + weight_decay * m[q];
       if (momentum != nullptr) {
         float v = momentum[i + q] * mu + gq;
         momentum[i + q] = v;
@@ -40,9 +51,11 @@ __global__ void sgd_step_kernel(float* __restrict__ master, const float* __restr
 // copy in the same pass (saves the transpose kernel's full re-read of the
 // bf16 tensor + a launch). Plain SGD + weight decay (momentum goes through
 // the 1-D kernel + separate transpose).
+template <bool SCALED>
 __global__ void sgd_step_t_kernel(float* __restrict__ master, const float* __restrict__ grad,
                                   __bf16* __restrict__ out, __bf16* __restrict__ outT,
-                                  int R, int C, float lr, float weight_decay) {
+                                  int R, int C, float lr, float weight_decay,
+                                  const float* __restrict__ gscale) {
   __shared__ __bf16 tile[64][64 + 2];
   int e = blockIdx.z;
   long base = (long)e * R * C;
@@ -57,6 +70,14 @@ __global__ void sgd_step_t_kernel(float* __restrict__ master, const float* __res
     f4 m1 = *(const f4*)(master + off + 4);
     f4 g0 = *(const f4*)(grad + off);
     f4 g1 = *(const f4*)(grad + off + 4);
+    if (SCALED) {
+      const float gs = *gscale;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        g0[q] = scaled_grad(g0[q], gs);
+        g1[q] = scaled_grad(g1[q], gs);
+      }
+    }
     bf16x8 o;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -89,9 +110,11 @@ __global__ void sgd_step_t_kernel(float* __restrict__ master, const float* __res
 // transposed bf16 copy in the same pass.
 // hash_u32 / round_sr moved to common.h (shared with the fused TN+SGD kernel)
 
+template <bool SCALED>
 __global__ void sgd_step_sr_t_kernel(__bf16* __restrict__ param, const float* __restrict__ grad,
                                      __bf16* __restrict__ paramT, int R, int C, float lr,
-                                     float weight_decay, unsigned seed) {
+                                     float weight_decay, unsigned seed,
+                                     const float* __restrict__ gscale) {
   __shared__ __bf16 tile[64][64 + 2];
   int e = blockIdx.z;
   long base = (long)e * R * C;
@@ -105,6 +128,14 @@ __global__ void sgd_step_sr_t_kernel(__bf16* __restrict__ param, const float* __
     bf16x8 p = *(const bf16x8*)(param + off);
     f4 g0 = *(const f4*)(grad + off);
     f4 g1 = *(const f4*)(grad + off + 4);
+    if (SCALED) {
+      const float gs = *gscale;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        g0[q] = scaled_grad(g0[q], gs);
+        g1[q] = scaled_grad(g1[q], gs);
+      }
+    }
     bf16x8 o;
     unsigned h = hash_u32((unsigned)(off & 0xFFFFFFFFu) ^ seed);
     unsigned h2 = hash_u32(h + 0x9e3779b9u);
@@ -195,29 +226,33 @@ __global__ void colsum_kernel(const __bf16* __restrict__ d, float* __restrict__ 
 
 extern "C" void lah_sgd_step(void* master, const void* grad, void* momentum,
                              void* out_bf16, long n, float lr, float mu,
-                             float weight_decay, hipStream_t stream) {
+                             float weight_decay, const void* gscale, hipStream_t stream) {
   long blocks = (n / 4 + 255) / 256;
   if (blocks > 2048) blocks = 2048;  // grid-stride (guide G11)
-  hipLaunchKernelGGL(sgd_step_kernel, dim3((unsigned)blocks), dim3(256), 0, stream,
+  auto kern = gscale != nullptr ? sgd_step_kernel<true> : sgd_step_kernel<false>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, stream,
                      (float*)master, (const float*)grad, (float*)momentum,
-                     (__bf16*)out_bf16, n, lr, mu, weight_decay);
+                     (__bf16*)out_bf16, n, lr, mu, weight_decay, (const float*)gscale);
 }
 
 extern "C" void lah_sgd_step_t(void* master, const void* grad, void* out, void* outT,
                                int E, int R, int C, float lr, float weight_decay,
-                               hipStream_t stream) {
+                               const void* gscale, hipStream_t stream) {
   dim3 grid(C / 64, R / 64, E), block(256);
-  hipLaunchKernelGGL(sgd_step_t_kernel, grid, block, 0, stream, (float*)master,
+  auto kern = gscale != nullptr ? sgd_step_t_kernel<true> : sgd_step_t_kernel<false>;
+  hipLaunchKernelGGL(kern, grid, block, 0, stream, (float*)master,
                      (const float*)grad, (__bf16*)out, (__bf16*)outT, R, C, lr,
-                     weight_decay);
+                     weight_decay, (const float*)gscale);
 }
 
 extern "C" void lah_sgd_step_sr_t(void* param, const void* grad, void* paramT, int E,
                                   int R, int C, float lr, float weight_decay,
-                                  unsigned seed, hipStream_t stream) {
+                                  unsigned seed, const void* gscale, hipStream_t stream) {
   dim3 grid(C / 64, R / 64, E), block(256);
-  hipLaunchKernelGGL(sgd_step_sr_t_kernel, grid, block, 0, stream, (__bf16*)param,
-                     (const float*)grad, (__bf16*)paramT, R, C, lr, weight_decay, seed);
+  auto kern = gscale != nullptr ? sgd_step_sr_t_kernel<true> : sgd_step_sr_t_kernel<false>;
+  hipLaunchKernelGGL(kern, grid, block, 0, stream, (__bf16*)param,
+                     (const float*)grad, (__bf16*)paramT, R, C, lr, weight_decay, seed,
+                     (const float*)gscale);
 }
 
 extern "C" void lah_transpose_bf16(const void* in, void* out, int E, int R, int C,

@@ -284,21 +284,37 @@ class FusedExpertSGD:
         step's pre-L compute — ~23 ms of SR traffic at the flagship)."""
         self._side_stream = stream
 
+    def gradients(self) -> list:
+        """The stack's weight gradients of this step (none before a backward):
+        what a norm over the whole model takes (ops.functional.grad_clip_scale)."""
+        st = self.stack
+        if self.fused_backward:
+            raise RuntimeError("fused_backward applies the gradients within the backward pass: "
+                               "there are none to clip")
+        return [st.main_grad_W1, st.main_grad_W2, st.main_grad_b1, st.main_grad_b2] if st.grad_ready else []
+
     @torch.no_grad()
-    def step(self) -> None:
+    def step(self, grad_scale: Optional[torch.Tensor] = None) -> None:
+        """grad_scale: a factor on the gradients, one fp32 number on the GPU
+        (grad_clip_scale's); the kernels apply it as they read them."""
+        if grad_scale is not None and self.fused_backward:
+            raise RuntimeError("fused_backward applied the gradients within the backward pass: "
+                               "they cannot be scaled any more")
         side = getattr(self, "_side_stream", None)
         if side is not None and self.stack.grad_ready:
             side.wait_stream(torch.cuda.current_stream())
+            if grad_scale is not None:
+                grad_scale.record_stream(side)
             with torch.cuda.stream(side):
-                self._step_body()
+                self._step_body(grad_scale)
             ev = torch.cuda.Event()
             ev.record(side)
             self.stack._opt_done_event = ev
             return
-        self._step_body()
+        self._step_body(grad_scale)
 
     @torch.no_grad()
-    def _step_body(self) -> None:
+    def _step_body(self, gs: Optional[torch.Tensor] = None) -> None:
         st = self.stack
         if not st.grad_ready:
             return
@@ -309,32 +325,32 @@ class FusedExpertSGD:
         elif self.stochastic_rounding:
             seed = self.sr_seed()
             _C.sgd_step_sr_t(st.W1c, st.main_grad_W1, st.W1t, self.lr,
-                             self.weight_decay, seed)
+                             self.weight_decay, seed, gs)
             _C.sgd_step_sr_t(st.W2c, st.main_grad_W2, st.W2t, self.lr,
-                             self.weight_decay, seed ^ 0x55555555)
+                             self.weight_decay, seed ^ 0x55555555, gs)
         elif self.momentum == 0.0:
             # fused path: one pass updates master + bf16 copy + bf16^T copy
             _C.sgd_step_t(st.W1.data, st.main_grad_W1, st.W1c, st.W1t,
-                          self.lr, self.weight_decay)
+                          self.lr, self.weight_decay, gs)
             _C.sgd_step_t(st.W2.data, st.main_grad_W2, st.W2c, st.W2t,
-                          self.lr, self.weight_decay)
+                          self.lr, self.weight_decay, gs)
         else:
             mom = self.momentum_bufs
             _C.sgd_step(st.W1.data.view(-1), st.main_grad_W1.view(-1), mom[0].view(-1),
-                        st.W1c.view(-1), self.lr, self.momentum, self.weight_decay)
+                        st.W1c.view(-1), self.lr, self.momentum, self.weight_decay, gs)
             _C.sgd_step(st.W2.data.view(-1), st.main_grad_W2.view(-1), mom[1].view(-1),
-                        st.W2c.view(-1), self.lr, self.momentum, self.weight_decay)
+                        st.W2c.view(-1), self.lr, self.momentum, self.weight_decay, gs)
             st.W1t.copy_(_C.transpose_bf16(st.W1c))
             st.W2t.copy_(_C.transpose_bf16(st.W2c))
         mom = self.momentum_bufs or [None] * 4
         scratch = torch.empty_like(st.W1_bias, dtype=torch.bfloat16)
         _C.sgd_step(st.W1_bias.data.view(-1), st.main_grad_b1.view(-1),
                     mom[2].view(-1) if mom[2] is not None else None,
-                    scratch.view(-1), self.lr, self.momentum, self.weight_decay)
+                    scratch.view(-1), self.lr, self.momentum, self.weight_decay, gs)
         scratch2 = torch.empty_like(st.W2_bias, dtype=torch.bfloat16)
         _C.sgd_step(st.W2_bias.data.view(-1), st.main_grad_b2.view(-1),
                     mom[3].view(-1) if mom[3] is not None else None,
-                    scratch2.view(-1), self.lr, self.momentum, self.weight_decay)
+                    scratch2.view(-1), self.lr, self.momentum, self.weight_decay, gs)
         st.b1_f32.copy_(st.W1_bias.data)
         st.b2_f32.copy_(st.W2_bias.data)
         st.zero_main_grads()
@@ -416,8 +432,16 @@ class ExpertAdam:
                 ("b1", st.W1_bias.data, st.W1_bias.grad),
                 ("b2", st.W2_bias.data, st.W2_bias.grad))
 
+    def gradients(self) -> list:
+        """The stack's weight gradients of this step, as FusedExpertSGD.gradients."""
+        if self.stack._gpu_state_ready and not self.stack.grad_ready:
+            return []
+        grads = [g for _, _, g in self._named_params_and_grads()]
+        return [] if any(g is None for g in grads) else grads
+
     @torch.no_grad()
-    def step(self) -> None:
+    def step(self, grad_scale: Optional[torch.Tensor] = None) -> None:
+        """grad_scale: a factor on the gradients, one number on their device."""
         st = self.stack
         if st._gpu_state_ready and not st.grad_ready:
             return
@@ -428,7 +452,8 @@ class ExpertAdam:
         b1, b2 = self.betas
         for name, p, g in named:
             m, v = self._mv(name, p)
-            adam_update_(p, g.float(), m, v, self.step_count, self.lr, b1, b2,
+            g = g.float() if grad_scale is None else g.float() * grad_scale
+            adam_update_(p, g, m, v, self.step_count, self.lr, b1, b2,
                          self.eps, self.weight_decay)
         if st._gpu_state_ready:
             # refresh bf16 compute copies + transposes + fp32 bias mirrors
@@ -467,6 +492,26 @@ class ExpertAdam:
             v[idx].copy_(mv["v"].to(v.device))
 
 
+class _AllToAllRows(torch.autograd.Function):
+    """All-to-all of uneven numbers of rows; the gradient goes the way back."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, send: list, recv: list, group):
+        ctx.send, ctx.recv, ctx.group = send, recv, group
+        out = x.new_empty(sum(recv), x.shape[1])
+        dist.all_to_all_single(out, x[: sum(send)].contiguous(), recv, send, group=group)
+        ctx.rows = x.shape[0]
+        return out
+
+    @staticmethod
+    def backward(ctx, grad: torch.Tensor):
+        out = grad.new_zeros(ctx.rows, grad.shape[1])
+        back = grad.new_empty(sum(ctx.send), grad.shape[1])
+        dist.all_to_all_single(back, grad.contiguous(), ctx.send, ctx.recv, group=ctx.group)
+        out[: back.shape[0]] = back
+        return out, None, None, None
+
+
 class _AllToAll(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: torch.Tensor, group):
@@ -499,8 +544,15 @@ class ExpertParallelMoE(nn.Module):
         group: Optional[object] = None,
         tokens_per_batch_hint: int = 8192,
         a2a_chunks: int = 1,
+        dropless: bool = False,
     ):
         super().__init__()
+        if dropless and a2a_chunks > 1:
+            raise ValueError("the chunked all-to-all is for capacity buffers: dropless needs a2a_chunks=1")
+        # dropless: no capacity — every chosen slot has a row, sorted by expert
+        # (ops/ragged.py). On one rank nothing waits for the host; over several
+        # the rows' numbers are read back once a call for the uneven all-to-all.
+        self.dropless = dropless
         self.d_model, self.ffn_dim = d_model, ffn_dim
         self.num_experts, self.k = num_experts, k
         self.capacity_factor = capacity_factor
@@ -587,6 +639,11 @@ class ExpertParallelMoE(nn.Module):
             logits = logits + self.router_noise_std * torch.randn_like(logits)
         with tm("moe_route"):
             topk_idx, topk_w, probs = Fops.gating_topk(logits, k)
+        if self.dropless:
+            y, counts = self._dropless(flat, topk_idx, topk_w, tm)
+            self.last_counts = counts
+            self.aux_loss = self._aux_losses(counts, probs, logits, T)
+            return y.reshape(*lead_shape, D).to(x.dtype)
         with torch.no_grad(), tm("moe_assign"):
             pos, counts, inv = Fops.assign_slots(topk_idx, E, C)
         with torch.no_grad():
@@ -638,6 +695,12 @@ class ExpertParallelMoE(nn.Module):
         with tm("moe_combine"):
             y = Fops.combine(ybuf, topk_idx, pos, topk_w, inv)
 
+        self.aux_loss = self._aux_losses(counts, probs, logits, T)
+        return y.reshape(*lead_shape, D).to(x.dtype)
+
+    def _aux_losses(self, counts: torch.Tensor, probs: torch.Tensor, logits: torch.Tensor,
+                    T: int) -> Optional[torch.Tensor]:
+        E, k = self.num_experts, self.k
         aux = None
         if self.aux_loss_coef > 0:
             f = (counts.float() / max(1, T * k)).detach()
@@ -649,8 +712,58 @@ class ExpertParallelMoE(nn.Module):
             z = torch.logsumexp(logits, dim=-1)
             z_loss = self.z_loss_coef * (z * z).mean()
             aux = z_loss if aux is None else aux + z_loss
-        self.aux_loss = aux
-        return y.reshape(*lead_shape, D).to(x.dtype)
+        return aux
+
+    def _dropless(self, flat: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor, tm):
+        """Rows sorted by expert -> (all-to-all ->) FFN over ragged groups -> back
+        -> weighted sum. Returns ([T, D], counts [E] of the chosen slots)."""
+        with torch.no_grad(), tm("moe_assign"):
+            if self.member_slots is not None:  # departed ranks' experts get no row
+                topk_idx = topk_idx.masked_fill(~self.expert_alive[topk_idx.long()], -1)
+            layout = Fops.ragged_layout(topk_idx, self.num_experts)
+            counts = layout.offsets[1:] - layout.offsets[:-1]
+        with tm("moe_dispatch"):
+            rows = Fops.ragged_gather(flat.to(torch.bfloat16 if flat.is_cuda else flat.dtype), layout)
+        if self.world_size == 1 and self.total_slots == 1:
+            with tm("moe_expert_ffn"):
+                y = Fops.ragged_ffn(rows, layout.offsets, self.experts)
+        else:
+            y = self._dropless_sharded(rows, counts, tm)
+        with tm("moe_combine"):
+            return Fops.ragged_combine(y, layout, topk_w), counts
+
+    def _dropless_sharded(self, rows: torch.Tensor, counts: torch.Tensor, tm) -> torch.Tensor:
+        """The FFN where experts are spread over ranks. Rows are sorted by expert,
+        so each rank's stand together; what arrives is sorted by (source, expert)
+        and is put in order of the expert here."""
+        W = self.world_size
+        members = self.member_slots if self.member_slots is not None else list(range(W))
+        P = self.num_experts // self.total_slots
+        with torch.no_grad():
+            sent = torch.cat([counts[s * P : (s + 1) * P] for s in members]).contiguous()
+            got = torch.empty_like(sent)
+            if W > 1:
+                dist.all_to_all_single(got, sent, group=self.group)
+            else:
+                got = sent
+            both = torch.stack([sent, got]).view(2, W, P).cpu()  # the one host read
+            send, recv = both.sum(-1).tolist()
+            ids = torch.arange(P, dtype=torch.int32).repeat(W).repeat_interleave(both[1].reshape(-1).long())
+            layout = Fops.ragged_layout(ids.to(rows.device).unsqueeze(1), P)
+        with tm("moe_a2a_fwd"):
+            if W > 1:
+                arrived = _AllToAllRows.apply(rows, send, recv, self.group)
+            else:
+                arrived = rows[: sum(recv)]
+        with tm("moe_expert_ffn"):
+            y = Fops.ragged_ffn(Fops.ragged_gather(arrived, layout), layout.offsets, self.experts)
+            y = Fops.ragged_ungather(y, layout)
+        with tm("moe_a2a_ret"):
+            if W > 1:
+                y = _AllToAllRows.apply(y, recv, send, self.group)
+        if y.shape[0] < rows.shape[0]:  # slots without an expert
+            y = torch.cat([y, y.new_zeros(rows.shape[0] - y.shape[0], y.shape[1])])
+        return y
 
     def _chunked_expert_pipeline(self, xbuf: torch.Tensor, W: int, P: int, C: int,
                                  D: int, n_chunks: int, tm) -> torch.Tensor:

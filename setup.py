@@ -22,6 +22,9 @@ ext = CUDAExtension(
         os.path.join(HIP_DIR, "optim.hip"),
         os.path.join(HIP_DIR, "attention.hip"),
         os.path.join(HIP_DIR, "ce.hip"),
+        os.path.join(HIP_DIR, "ragged_layout.hip"),
+        os.path.join(HIP_DIR, "ragged_gemm.hip"),
+        os.path.join(HIP_DIR, "clip.hip"),
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
