@@ -9,8 +9,7 @@
 // launch can be captured. No row is padded: a row past an expert's end is
 // loaded as zeros (the buffer descriptor's range check) and never stored.
 //
-// One tile kernel serves the three products. P is the operand whose index
-// becomes the output's fast axis, Q the other one:
+// P is the operand whose index becomes the output's fast axis, Q the other one:
 //             P                         Q                    contraction
 //   NT fwd    W[e]  [N][K]   (KC)       x   rows  (KC)       K
 //   NN dx     W[e]  [Kc][N]  (KS)       dP  rows  (KC)       Kc
@@ -18,15 +17,25 @@
 // KC: the contraction is the operand's fast axis; a fragment is one 16-byte LDS
 // read. KS: it is the slow axis; the fragment is read transposed from LDS
 // (ds_read_b64_tr_b16), so no transposed copy of a weight is needed.
+//
+// A block is 4 waves on a tile of 128 Q by 256 P, a wave 64 by 128: 128
+// accumulators a lane, so that two blocks share a CU and one's epilogue (gelu is
+// as long as a third of the products at K = 1024) hides under the other's products.
 #include "common.h"
+#include <type_traits>
+#include <utility>
 
-#define RBK 32  // contraction steps of a stage
+#define RBK 32   // contraction steps of a phase of KS operands
+#define RBN 256  // P's side of a tile
+#define RBM 128  // Q's side
+#define RT 256   // threads
 
 enum { R_NT = 0, R_NN = 1, R_TN = 2 };
 enum { R_PLAIN = 0, R_GELU = 1, R_GELU_DER = 2, R_MUL = 3 };  // forward epilogues
 enum { R_F32 = 0, R_F32_ACC = 1, R_BF16 = 2 };                // dW outputs
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 #define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
 
 LAH_DEVINL unsigned lds_addr(const void* p) {
@@ -34,13 +43,12 @@ LAH_DEVINL unsigned lds_addr(const void* p) {
 }
 
 // Buffer descriptor of `bytes` from p: loads past them give zeros.
-LAH_DEVINL i32x4 make_rsrc(const void* p, long bytes) {
+LAH_DEVINL i32x4 make_rsrc(const void* p, int bytes) {
   const unsigned long long a = (unsigned long long)p;
-  const long b = bytes < 0 ? 0 : (bytes > 0x7fffffffL ? 0x7fffffffL : bytes);
   i32x4 r;
   r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
   r[1] = __builtin_amdgcn_readfirstlane((int)(unsigned)((a >> 32) & 0xffff));
-  r[2] = __builtin_amdgcn_readfirstlane((int)b);
+  r[2] = __builtin_amdgcn_readfirstlane(bytes);
   r[3] = 0x00027000;
   return r;
 }
@@ -64,15 +72,33 @@ LAH_DEVINL void wait_and_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// LDS places of 16-byte chunks, so that the 16 lanes that read together hit 16
-// different places mod 256 bytes (64 banks):
-//  KC tile [rows][32]: 4 chunks a row; the chunk is XORed with two row bits. P's
-//  rows come in steps of FN*4 (see p_row), so P takes its two bits there.
+LAH_DEVINL void wait_reads_and_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+LAH_DEVINL void barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+// LDS places of 16-byte chunks, so that the 16 lanes that are served together hit
+// 16 different places mod 256 bytes (64 banks).
+//  KC tile [rows][64], 8 chunks a row: a 16-byte read serves quads of lanes q = 0, 3
+//  of one 16 and 1, 2 of the next together, and the others. Chunks are XORed with
+//  0 2 3 1 by the quad's row bits, and the row's second bit on top (counted: no
+//  conflict; the quad's bits themselves conflict two ways).
 //  KS tile [32][cols]: a transposed read takes 2 chunks of each of 8 rows
 //  {0..3, 8..11} (+4, +16); three row bits move the chunk pair.
 template <int SHIFT>
-LAH_DEVINL int kc_swz(int row) { return (row >> SHIFT) & 3; }
+LAH_DEVINL int kc_swz(int row) {
+  const int q = (row >> SHIFT) & 3;
+  return ((row & 2) << 1) | (((q << 1) ^ q) & 2) | (q >> 1);
+}
 LAH_DEVINL int ks_swz(int row) { return ((row & 3) | ((row >> 1) & 4)) << 1; }
+
+// Fragment of a KS tile: lane i of 16 gets column base + i at rows 8g .. 8g + 7.
+LAH_DEVINL bf16x8 read_ks(const __bf16* tile, int cols, int base, int lane) {
+  const int l15 = lane & 15, r = (lane >> 4) * 8 + (l15 >> 2), col = base + 4 * (l15 & 3);
+  const int c0 = ((col >> 3) ^ ks_swz(r)) * 8 + (col & 7);
+  const int c1 = ((col >> 3) ^ ks_swz(r + 4)) * 8 + (col & 7);
+  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, tile + r * cols + c0));
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, tile + (r + 4) * cols + c1));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 
 LAH_DEVINL float gelu_of(float x) {  // x * sigmoid(2u): one exp2, one reciprocal
   const float x2 = x * x;
@@ -121,299 +147,827 @@ struct RaggedArgs {
   int bias_bf16;     // of bias, or of db
 };
 
-template <int KIND, int EPI, int WN, int WM, int FN, int FM, int STAGES>
-__launch_bounds__(WN * WM * 64, 2) __global__ void ragged_gemm_kernel(RaggedArgs a) {
-  constexpr int BN = WN * FN * 16, BM = WM * FM * 16, T = WN * WM * 64;
-  constexpr bool P_KC = KIND == R_NT, Q_KC = KIND != R_TN;
-  constexpr int PL = BN * RBK / 8 / T, QL = BM * RBK / 8 / T;  // loads a thread and stage
-  constexpr int STAGE = (BN + BM) * RBK;                       // elements
-  constexpr int PSHIFT = FN == 8 ? 5 : 4;                      // log2(FN * 4)
-  static_assert(BN * RBK / 8 % T == 0 && BM * RBK / 8 % T == 0, "whole loads");
-  static_assert(FN == 8 || FN == 4, "p_row and its swizzle");
-  __shared__ __attribute__((aligned(16))) __bf16 smem[STAGES * STAGE];
+// Blocks go to the 8 XCDs in turn: of each 512, the 64 that share one XCD (two a
+// CU) take 64 neighbouring tiles, whose operands then share its L2.
+LAH_DEVINL int xcd_tile() {
+  const int L = blockIdx.x;
+  return L < ((int)gridDim.x & ~511) ? (L & ~511) | ((L & 7) << 6) | ((L >> 3) & 63) : L;
+}
+
+// rows [lo, hi) of expert e, whatever the offsets hold
+LAH_DEVINL void expert_rows(const RaggedArgs& a, int e, long* lo, long* hi) {
+  *lo = e == 0 ? 0 : min((long)max(a.offsets[e], 0), a.R);
+  *hi = e == a.E ? a.R : min(max((long)a.offsets[e + 1], *lo), a.R);
+}
+
+#define MFMA(a, b, c) __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0)
+
+// ---------------------------------------------------------------------------
+// forward (NT) and dx (NN): rows of Q against one expert's weight
+//
+// A stage is 64 contraction steps, so that KC rows are whole 128-byte lines (at 32
+// the same loads are twice the requests: 740 against 1000 TFLOP/s). It runs in two
+// phases of 32 MFMAs a wave: NT takes half of P's rows in each (Q's fragments stay
+// in registers), NN half of the contraction. P rides in a ring of 3 half stages, Q
+// in 2 whole ones: 80 KB, just two blocks a CU, and every load has two phases to land.
+// ---------------------------------------------------------------------------
+template <int KIND, int EPI>
+__launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
+  constexpr bool P_KC = KIND == R_NT;
+  constexpr int SLOT = 8192;  // elements: 128 x 64 (KC) or 32 x 256 (KS)
+  __shared__ __attribute__((aligned(16))) __bf16 smem[5 * SLOT];
 
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = wave % WN, wm = wave / WN;
+  const int wn = wave & 1, wm = wave >> 1;
 
-  // Blocks go to the 8 XCDs in turn: of each 512, the 64 that share one XCD
-  // (two a CU) take 64 neighbouring tiles, whose operands then share its L2.
-  int L = blockIdx.x;
-  if (L < ((int)gridDim.x & ~511)) L = (L & ~511) | ((L & 7) << 6) | ((L >> 3) & 63);
-  const int NT = cdiv(a.N, BN);
+  const int L = xcd_tile(), NT = cdiv(a.N, RBN);
+  const int e = __builtin_amdgcn_readfirstlane(find_expert<RBM>(a.offsets, a.E, L / NT));
+  long lo, hi;
+  expert_rows(a, e, &lo, &hi);
+  const int s0 = (int)(lo / RBM) + e, slots = (int)(hi / RBM) - (int)(lo / RBM) + 1;
+  // 8 M-tiles by all N-tiles at a time: neighbours share rows and weights
+  const int q = L - s0 * NT;
+  const int first = q / (8 * NT) * 8, size = min(slots - first, 8), in = q % (8 * NT);
+  const int m0 = (first + in % size) * RBM, n0 = in / size * RBN;
+  const long row0 = lo + m0;
+  if (q < 0 || size <= 0 || row0 >= hi || n0 >= a.N) return;  // also where offsets do not ascend
+  const int rows = (int)min(hi - row0, (long)RBM);
+  const int steps = e == a.E ? 0 : cdiv(a.K, 64);
 
-  int e, m0, n0, rows, steps;
-  long row0;
-  if (KIND == R_TN) {
-    const int MT = cdiv(a.M, BM);
-    e = L / (MT * NT);
-    const int q = L % (MT * NT);
-    const int first = q / (8 * NT) * 8, size = min(MT - first, 8), in = q % (8 * NT);
-    m0 = (first + in % size) * BM;
-    n0 = in / size * BN;
-    const long lo = e == 0 ? 0 : min((long)max(a.offsets[e], 0), a.R);
-    const long hi = min(max((long)a.offsets[e + 1], lo), a.R);
-    row0 = lo;
-    rows = (int)(hi - lo);
-    steps = cdiv(rows, RBK);
-  } else {
-    e = find_expert<BM>(a.offsets, a.E, L / NT);
-    e = __builtin_amdgcn_readfirstlane(e);
-    const long lo = e == 0 ? 0 : min((long)max(a.offsets[e], 0), a.R);
-    const long hi = e == a.E ? a.R : min(max((long)a.offsets[e + 1], lo), a.R);
-    const int s0 = (int)(lo / BM) + e, slots = (int)(hi / BM) - (int)(lo / BM) + 1;
-    // 8 M-tiles by all N-tiles at a time: neighbours share rows and weights
-    const int q = L - s0 * NT;
-    const int first = q / (8 * NT) * 8, size = min(slots - first, 8), in = q % (8 * NT);
-    m0 = (first + in % size) * BM;
-    n0 = in / size * BN;
-    row0 = lo + m0;
-    if (q < 0 || size <= 0 || row0 >= hi || n0 >= a.N) return;  // also where offsets do not ascend
-    rows = (int)min(hi - row0, (long)BM);
-    steps = e == a.E ? 0 : cdiv(a.K, RBK);
-  }
-
-  // ---- staging: each thread's byte offsets in its tile are the same in every step
-  const __bf16 *Pb, *Qb;
-  long pbytes, qbytes;  // from the base to the end of what may be read
-  long pstep, qstep;    // elements from one stage to the next
-  if (KIND == R_NT) {
-    Pb = a.P + ((long)e * a.N + n0) * a.K;
-    pbytes = (long)min(a.N - n0, BN) * a.K * 2;
-    pstep = RBK;
-  } else if (KIND == R_NN) {
-    Pb = a.P + (long)e * a.K * a.N + n0;
-    pbytes = ((long)a.K * a.N - n0) * 2;
-    pstep = (long)RBK * a.N;
-  } else {
-    Pb = a.P + row0 * a.N + n0;
-    pbytes = ((long)rows * a.N - n0) * 2;
-    pstep = (long)RBK * a.N;
-  }
-  if (KIND == R_TN) {
-    Qb = a.Q + row0 * a.M + m0;
-    qbytes = ((long)rows * a.M - m0) * 2;
-    qstep = (long)RBK * a.M;
-  } else {
-    Qb = a.Q + row0 * a.K;
-    qbytes = (long)rows * a.K * 2;
-    qstep = RBK;
-  }
-  unsigned pv[PL], qv[QL];
-  int pc[PL], qc[QL];  // KC: the chunk's first contraction index
+  // ---- staging: a thread's byte offsets in a tile are the same in every stage
+  const __bf16* Pb = a.P + ((long)e * a.N * a.K + (P_KC ? (long)n0 * a.K : n0));
+  const __bf16* Qb = a.Q + row0 * a.K;
+  // bytes from the base to the end of what may be read (below 2^31: N * K < 2^30, K < 2^21)
+  const int pbytes = P_KC ? min(a.N - n0, RBN) * a.K * 2 : 0, qbytes = rows * a.K * 2;
+  unsigned pv[4], qv[4];
+  int cc[4];  // KC: a chunk's first contraction index
 #pragma unroll
-  for (int i = 0; i < PL; ++i) {
-    const int idx = i * T + tid;
-    if (P_KC) {
-      const int r = idx >> 2, c = (idx & 3) ^ kc_swz<PSHIFT>(r);
-      pv[i] = (unsigned)((long)r * a.K * 2 + c * 16);
-      pc[i] = c * 8;
+  for (int i = 0; i < 4; ++i) {
+    const int idx = i * RT + tid;
+    const int r = idx >> 3, c = (idx & 7) ^ kc_swz<2>(r);
+    qv[i] = (unsigned)(r * a.K + c * 8) * 2;
+    cc[i] = c * 8;
+    if (P_KC) {  // half h has rows 128 wn + 32 q + 16 h + ..: 16 of every 32
+      const int pc = (idx & 7) ^ kc_swz<4>(r);
+      pv[i] = (unsigned)(((r >> 4) * 32 + (r & 15)) * a.K + pc * 8) * 2;
     } else {
-      const int r = idx / (BN / 8), c = (idx % (BN / 8)) ^ ks_swz(r);
-      pv[i] = (unsigned)((long)r * a.N * 2 + c * 16);
+      const int kr = idx >> 5, pc = (idx & 31) ^ ks_swz(kr);
+      pv[i] = (unsigned)(kr * a.N + pc * 8) * 2;
     }
   }
+  int pcc[4];
 #pragma unroll
-  for (int i = 0; i < QL; ++i) {
-    const int idx = i * T + tid;
-    if (Q_KC) {
-      const int r = idx >> 2, c = (idx & 3) ^ kc_swz<2>(r);
-      qv[i] = (unsigned)((long)r * a.K * 2 + c * 16);
-      qc[i] = c * 8;
-    } else {
-      const int r = idx / (BM / 8), c = (idx % (BM / 8)) ^ ks_swz(r);
-      qv[i] = (unsigned)((long)r * a.M * 2 + c * 16);
-    }
-  }
+  for (int i = 0; i < 4; ++i) pcc[i] = ((i * RT + tid) & 7 ^ kc_swz<4>((i * RT + tid) >> 3)) * 8;
   const unsigned lds0 = lds_addr(smem) + wave * 1024;
 
-  auto stage = [&](int t, int buf) {
-    const unsigned to = lds0 + buf * STAGE * 2;
-    const i32x4 rp = make_rsrc(Pb + t * pstep, pbytes - t * pstep * 2);
-    const i32x4 rq = make_rsrc(Qb + t * qstep, qbytes - t * qstep * 2);
-    // chunks past the contraction's end, which only a KC tile can hold, give zeros
-    const int left = KIND == R_TN ? RBK : a.K - t * RBK;
+  auto stage_p = [&](int p) {  // phase p's part, to slot p % 3
+    const int t = p >> 1, h = p & 1;
+    const unsigned to = lds0 + (p % 3) * (SLOT * 2);
+    if (P_KC) {
+      const int skip = h * 16 * a.K + t * 64;
+      const i32x4 r = make_rsrc(Pb + skip, max(pbytes - skip * 2, 0));  // few columns: no second half
+      const int left = a.K - t * 64;
 #pragma unroll
-    for (int i = 0; i < PL; ++i)
-      lds_load16(rp, P_KC && pc[i] >= left ? OOB_OFFSET : pv[i], to + i * T * 16);
+      for (int i = 0; i < 4; ++i) lds_load16(r, pcc[i] >= left ? OOB_OFFSET : pv[i], to + i * RT * 16);
+    } else {
+      const int left = max(min(a.K - p * RBK, RBK), 0);
+      const i32x4 r = make_rsrc(Pb + (long)p * RBK * a.N, left > 0 ? (left * a.N - n0) * 2 : 0);
 #pragma unroll
-    for (int i = 0; i < QL; ++i)
-      lds_load16(rq, Q_KC && qc[i] >= left ? OOB_OFFSET : qv[i], to + BN * RBK * 2 + i * T * 16);
+      for (int i = 0; i < 4; ++i) lds_load16(r, pv[i], to + i * RT * 16);
+    }
+  };
+  auto stage_q = [&](int t) {
+    const unsigned to = lds0 + (3 + (t & 1)) * (SLOT * 2);
+    const i32x4 r = make_rsrc(Qb + t * 64, qbytes - t * 128);
+    const int left = a.K - t * 64;  // chunks past the contraction's end give zeros
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds_load16(r, cc[i] >= left ? OOB_OFFSET : qv[i], to + i * RT * 16);
   };
 
-  f32x4 acc[FN][FM];
-  f32x4 dbacc[KIND == R_TN ? FM : 1];
+  f32x4 acc[8][4];
 #pragma unroll
-  for (int i = 0; i < FN; ++i)
+  for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < FM; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 4; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+
+  // P's fragment i, lane l15 is tile row 128 wn + 32 (l15 / 4) + 4 i + l15 % 4: a
+  // lane's results in D rows 4g .. 4g+3 of all 8 are then 32 neighbouring outputs.
+  const int prow = wn * 64 + (l15 >> 2) * 16 + (l15 & 3);  // in a half's slot, + 4 (i & 3)
+  const int qrow = wm * 64 + l15;
+  auto read_q = [&](int t, int j, int kk) {
+    const int r = qrow + j * 16;
+    return *(const bf16x8*)(smem + (3 + (t & 1)) * SLOT + r * 64 + ((kk * 4 + g) ^ kc_swz<2>(r)) * 8);
+  };
+  auto read_p_kc = [&](int p, int i, int kk) {
+    const int r = prow + i * 4;
+    return *(const bf16x8*)(smem + (p % 3) * SLOT + r * 64 + ((kk * 4 + g) ^ kc_swz<4>(r)) * 8);
+  };
+
+  if (steps > 0) {
+    stage_p(0);
+    stage_q(0);
+    stage_p(1);
+  }
+  for (int t = 0; t < steps; ++t) {
+    const bool more = t + 1 < steps;
+    bf16x8 qf[4][2];
+    // the phase's loads have landed; all waves are past their reads of what is refilled now
+    wait_and_barrier<4>();
+    if (more) {
+      stage_p(2 * t + 2);
+      stage_q(t + 1);
+    }
 #pragma unroll
-  for (int j = 0; j < (KIND == R_TN ? FM : 1); ++j) dbacc[j] = {0.f, 0.f, 0.f, 0.f};
-  const bool with_db = KIND == R_TN && a.db != nullptr && n0 == 0 && wn == 0;
-  bf16x8 ones;
+    for (int j = 0; j < 4; ++j) {
+      qf[j][0] = read_q(t, j, 0);
+      if (P_KC) qf[j][1] = read_q(t, j, 1);
+    }
+    bf16x8 pf[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      pf[i] = P_KC ? read_p_kc(2 * t, i & 3, i >> 2)
+                   : read_ks(smem + (2 * t) % 3 * SLOT, RBN, wn * 128 + i * 16, lane);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (P_KC) acc[i & 3][j] = MFMA(pf[i], qf[j][i >> 2], acc[i & 3][j]);
+        else acc[i][j] = MFMA(pf[i], qf[j][0], acc[i][j]);
+      }
+    if (more) {
+      wait_and_barrier<8>();
+      stage_p(2 * t + 3);
+    } else {
+      wait_and_barrier<0>();
+    }
+    if (!P_KC) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) qf[j][1] = read_q(t, j, 1);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      pf[i] = P_KC ? read_p_kc(2 * t + 1, i & 3, i >> 2)
+                   : read_ks(smem + (2 * t + 1) % 3 * SLOT, RBN, wn * 128 + i * 16, lane);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (P_KC) acc[4 + (i & 3)][j] = MFMA(pf[i], qf[j][i >> 2], acc[4 + (i & 3)][j]);
+        else acc[i][j] = MFMA(pf[i], qf[j][1], acc[i][j]);
+      }
+  }
+
+  // ---- epilogue: lane (l15, g) holds output row 16 j + l15
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = wm * 64 + j * 16 + l15;
+    if (r >= rows) continue;
+    const long at = (row0 + r) * a.N;
+    constexpr int STEP = P_KC ? 8 : 4;  // neighbouring outputs stored at once
+#pragma unroll
+    for (int i0 = 0; i0 < 8; i0 += STEP / 4) {
+      const int n = n0 + wn * 128 + (P_KC ? g * 32 + i0 * 4 : i0 * 16 + g * 4);
+      if (n >= a.N) continue;
+      float v[STEP];
+#pragma unroll
+      for (int x = 0; x < STEP; ++x) v[x] = acc[i0 + x / 4][j][x & 3];
+      if (KIND == R_NT && a.bias != nullptr && e < a.E) {
+        if (a.bias_bf16) {
+          const bf16x8 b = *(const bf16x8*)((const __bf16*)a.bias + (long)e * a.N + n);
+#pragma unroll
+          for (int x = 0; x < STEP; ++x) v[x] += bf2f(b[x & 7]);
+        } else {
+#pragma unroll
+          for (int h = 0; h < STEP; h += 4) {
+            const f32x4 b = *(const f32x4*)((const float*)a.bias + (long)e * a.N + n + h);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[h + x] += b[x];
+          }
+        }
+      }
+      typedef __attribute__((ext_vector_type(STEP))) __bf16 outv;
+      outv o, d;
+      if (EPI == R_MUL) d = *(const outv*)(a.der + at + n);
+#pragma unroll
+      for (int x = 0; x < STEP; ++x) {
+        if (EPI == R_GELU) {
+          o[x] = f2bf(gelu_of(v[x]));
+        } else if (EPI == R_GELU_DER) {
+          float y, s;
+          gelu_and_slope(v[x], &y, &s);
+          o[x] = f2bf(y);
+          d[x] = f2bf(s);  // the slope, in the outputs' type: one rounding of dP more
+        } else if (EPI == R_MUL) {
+          o[x] = f2bf(v[x] * bf2f(d[x]));
+        } else {
+          o[x] = f2bf(v[x]);
+        }
+      }
+      *(outv*)((__bf16*)a.C + at + n) = o;
+      if (EPI == R_GELU_DER) *(outv*)(a.der + at + n) = d;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: 256 x 256 tiles, one persistent block of 4 waves a CU
+//
+// A wave has 128 x 128 of the tile, 256 accumulators a lane, and its SIMD to itself.
+// Against 8 waves of 64 x 128 that is a third fewer LDS reads and half the scalar
+// work a product, and what bounds large products on this card is power: at 4 x 8192
+// rows, K = N = 4096, 8 waves ran 52 % of the MFMA cycles at 2.05 GHz.
+//
+// A CU has room for one such tile, so nothing else could hide its first loads and
+// last stores: the block runs through a list of tiles and loads two stages ahead,
+// into the next tile where the present one ends; stores are left in flight. A stage
+// is 64 contraction steps of P and Q (32 KB each, two stages in LDS), in halves of
+// 32: while one half is multiplied, the fragments of the next are read, one or two
+// LDS reads or loads in the gap behind each MFMA. Behind a stage's first quarter its
+// place is free (a barrier, where no read is out) and is loaded again; a second
+// barrier, before the last quarter, says that the next stage has landed: loads have
+// a stage and a half (at a stage, the misses of L2 were waited for: 10 % more time).
+// ---------------------------------------------------------------------------
+// ---------------------------------------------------------------------------
+#define BT 256
+#define BM 256
+#define BN 256
+#define BSLOT 16384  // elements of one operand's stage
+
+// M-tiles of all experts in order: table[0] = their number, then {expert, first
+// row, rows, 0}. Rows of nobody come last, as expert E.
+__launch_bounds__(1024) __global__ void ragged_tiles_kernel(const int* __restrict__ offsets, int E, long R,
+                                                            int4* __restrict__ table) {
+  __shared__ int start[4098];
+  __shared__ int wsum[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int PER = 5;  // E + 1 <= 4097 groups
+  int c[PER], sum = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int e = tid * PER + j;
+    c[j] = 0;
+    if (e <= E) {
+      const long lo = e == 0 ? 0 : min((long)max(offsets[e], 0), R);
+      const long hi = e == E ? R : min(max((long)offsets[e + 1], lo), R);
+      c[j] = (int)((hi - lo + BM - 1) / BM);
+    }
+    sum += c[j];
+  }
+  int inc = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(inc, d, 64);
+    if (lane >= d) inc += v;
+  }
+  if (lane == 63) wsum[wave] = inc;
+  __syncthreads();
+  int at = inc - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    at += w < wave ? wsum[w] : 0;
+    total += wsum[w];
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (tid * PER + j <= E) start[tid * PER + j] = at;
+    at += c[j];
+  }
+  // where offsets do not ascend, groups overlap: no more tiles than the table has room for
+  const int most = (int)min((long)total, R / BM + E + 1);
+  if (tid == 0) table[0] = make_int4(most, 0, 0, 0);
+  __syncthreads();
+  for (int i = tid; i < most; i += 1024) {
+    int lo_e = 0, hi_e = E;  // the last group that starts at or before tile i has it
+    while (lo_e < hi_e) {
+      const int mid = (lo_e + hi_e + 1) >> 1;
+      if (start[mid] <= i) lo_e = mid;
+      else hi_e = mid - 1;
+    }
+    const int e = lo_e;
+    const long lo = e == 0 ? 0 : min((long)max(offsets[e], 0), R);
+    const long hi = e == E ? R : min(max((long)offsets[e + 1], lo), R);
+    const long row0 = lo + (long)(i - start[e]) * BM;
+    table[1 + i] = make_int4(e, (int)row0, (int)max(min(hi - row0, (long)BM), 0l), 0);
+  }
+}
+
+// The accumulators of a wave that has its SIMD to itself fill the accumulation
+// registers; the compiler's own products move them about (four copies before each, with
+// the branches below). In asm it cannot see how long their results take: whatever else
+// touches them stands behind settle(), 32 cycles.
+LAH_DEVINL void mfma_acc(f32x4& c, const bf16x8& a, const bf16x8& b) {
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+// a few more, in the other registers
+LAH_DEVINL void mfma_vgpr(f32x4& c, const bf16x8& a, const bf16x8& b) {
+  asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+}
+LAH_DEVINL void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+// the value is in its accumulation registers here, and read or written beyond
+LAH_DEVINL void pin_acc(f32x4& c) { asm volatile("" : "+a"(c)); }
+
+LAH_DEVINL void pin_vgpr(f32x4& c) { asm volatile("" : "+v"(c)); }
+
+// as lds_load16, to a place at a fixed distance
+template <int AT>
+LAH_DEVINL void lds_load16_at(i32x4 rsrc, unsigned voff, unsigned lds) {
+  asm volatile(
+      "s_add_u32 m0, %0, %3\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      ::"s"(lds), "v"(voff), "s"(rsrc), "n"(AT)
+      : "memory", "scc");
+}
+LAH_DEVINL bf16x8 lds_read16(unsigned at, int off) {
+  return *(__attribute__((address_space(3))) const bf16x8*)(at + off);
+}
+LAH_DEVINL bf16x8 lds_read_tr(unsigned at, int off, int four_rows) {
+  typedef __attribute__((address_space(3))) bf16x4* place;
+  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((place)(at + off));
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((place)(at + off + four_rows));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <typename F, int... X>
+LAH_DEVINL void each_of(F&& f, std::integer_sequence<int, X...>) {
+  (f(std::integral_constant<int, X>()), ...);
+}
+template <typename F>
+LAH_DEVINL void each16(F&& f) { each_of(f, std::make_integer_sequence<int, 16>()); }
+
+struct BigTile {
+  int e, rows, steps, m0, n0;
+  long row0;
+};
+
+template <int KIND, int EPI>
+__launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const int4* __restrict__ table) {
+  constexpr bool P_KC = KIND == R_NT, Q_KC = KIND != R_TN;
+  __shared__ __attribute__((aligned(16))) __bf16 smem[4 * BSLOT];
+  __shared__ __attribute__((aligned(16))) float bias_lds[4][BN];
+
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave & 1, wm = wave >> 1;
+
+  const int NT = cdiv(a.N, BN);
+  // M-tiles of one expert, or of all
+  const int MT = KIND == R_TN ? cdiv(a.M, BM) : __builtin_amdgcn_readfirstlane(table[0].x);
+  const int tiles = KIND == R_TN ? a.E * MT * NT : MT * NT;
+  // 32 neighbouring tiles at a time on the 32 CUs of an XCD (blocks go to XCDs in turn)
+  const int stride = gridDim.x;
+  const int mine = stride % 256 == 0 ? (blockIdx.x & ~255) | ((blockIdx.x & 7) << 5) | ((blockIdx.x >> 3) & 31)
+                                     : (int)blockIdx.x;
+
+  auto decode = [&](int L) {  // 8 M-tiles by all N-tiles at a time
+    BigTile w;
+    int q = L;
+    if (KIND == R_TN) {
+      w.e = L / (MT * NT);
+      q = L % (MT * NT);
+    }
+    const int first = q / (8 * NT) * 8, size = min(MT - first, 8), in = q % (8 * NT);
+    const int m = first + in % size;
+    w.n0 = in / size * BN;
+    if (KIND == R_TN) {
+      long lo, hi;
+      expert_rows(a, w.e, &lo, &hi);
+      w.row0 = lo;
+      w.rows = (int)(hi - lo);
+      w.m0 = m * BM;
+      w.steps = max(cdiv(w.rows, 64), 1);
+    } else {
+      const int4 t = table[1 + m];
+      w.e = t.x;
+      w.row0 = t.y;
+      w.rows = t.z;
+      w.m0 = 0;
+      w.steps = w.e == a.E ? 1 : cdiv(a.K, 64);
+    }
+    w.e = __builtin_amdgcn_readfirstlane(w.e);
+    w.rows = __builtin_amdgcn_readfirstlane(w.rows);
+    w.steps = __builtin_amdgcn_readfirstlane(w.steps);
+    w.row0 = (long)(unsigned)__builtin_amdgcn_readfirstlane((int)w.row0);
+    return w;
+  };
+
+  // ---- staging: a thread's byte offsets are the same in every stage
+  unsigned pv0[8], qv0[8];
+  const int pr = P_KC ? tid >> 3 : tid >> 5, qr = Q_KC ? tid >> 3 : tid >> 4;
+  const int pc = P_KC ? ((tid & 7) ^ kc_swz<3>(pr)) * 8 : 0;
+  const int qc = Q_KC ? ((tid & 7) ^ kc_swz<2>(qr)) * 8 : ((tid & 15) ^ ks_swz(qr)) * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    pv0[i] = P_KC ? (unsigned)((pr + i * 32) * a.K + pc) * 2
+                 : (unsigned)((pr + i * 8) * a.N + ((tid & 31) ^ ks_swz(pr + i * 8)) * 8) * 2;
+    // KS: two tiles [64][128] beside each other
+    qv0[i] = Q_KC ? (unsigned)((qr + i * 32) * a.K + qc) * 2
+                 : (unsigned)((qr + (i & 3) * 16) * a.M + (i >> 2) * 128 + qc) * 2;
+  }
+  const unsigned lds0 = lds_addr(smem) + wave * 1024;
+  const unsigned bias0 = lds_addr(bias_lds);
+
+  // The stage that is loaded next: descriptors, contraction steps left, place. Within a
+  // tile they move on by a few scalar additions.
+  const char *pat = nullptr, *qat = nullptr;
+  int pbytes = 0, qbytes = 0, left = 0;
+  unsigned to = lds0;
+  const long pstep = P_KC ? 128 : 128L * a.N, qstep = Q_KC ? 128 : 128L * a.M;  // bytes
+  unsigned pv[8], qv[8];  // offsets in use: past everything where the contraction has ended
+  auto mask_offsets = [&]() {  // KC: chunks past the contraction's end give zeros
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      pv[i] = P_KC && pc >= left ? OOB_OFFSET : pv0[i];
+      qv[i] = Q_KC && qc >= left ? OOB_OFFSET : qv0[i];
+    }
+  };
+  auto set_bytes = [&](const BigTile& w) {  // KS: bytes that may be read
+    const int l = max(min(left, 64), 0);
+    if (!P_KC) pbytes = max((l * a.N - w.n0) * 2, 0);
+    if (!Q_KC) qbytes = max((l * a.M - w.m0) * 2, 0);
+  };
+  auto point_at = [&](const BigTile& w) {  // a tile's first stage
+    if (KIND == R_TN) {
+      left = w.rows;
+      pat = (const char*)(a.P + w.row0 * a.N + w.n0);
+      qat = (const char*)(a.Q + w.row0 * a.M + w.m0);
+    } else {
+      left = w.e == a.E ? 0 : a.K;  // rows of nobody: all zeros
+      qat = (const char*)(a.Q + w.row0 * a.K);
+      qbytes = left > 0 ? w.rows * a.K * 2 : 0;
+      pat = (const char*)(a.P + (long)w.e * a.K * a.N + (P_KC ? (long)w.n0 * a.K : w.n0));
+      pbytes = left > 0 ? min(a.N - w.n0, BN) * a.K * 2 : 0;
+    }
+    set_bytes(w);
+    if ((P_KC || Q_KC) && a.K % 64 != 0) mask_offsets();
+  };
+  auto point_on = [&](const BigTile& w) {
+    left -= 64;
+    pat += pstep;
+    qat += qstep;
+    if (P_KC) pbytes -= 128;
+    if (Q_KC) qbytes -= 128;
+    if (left < 64) {
+      set_bytes(w);
+      if (P_KC || Q_KC) mask_offsets();
+    }
+  };
+  auto load_p = [&](auto i) {
+    constexpr int I = decltype(i)::value;
+    lds_load16_at<I * BT * 16>(make_rsrc(pat, pbytes), pv[I], to);
+  };
+  auto load_q = [&](auto i) {
+    constexpr int I = decltype(i)::value;
+    lds_load16_at<BSLOT * 2 + I * BT * 16>(make_rsrc(qat, qbytes), qv[I], to);
+  };
+  // a tile's bias, with its first stage, by the first wave: loads are up to two tiles ahead
+  auto stage_bias = [&](const BigTile& w, int turn) {
+    if (KIND == R_NT && a.bias != nullptr && wave == 0) {
+      const int size = a.bias_bf16 ? 2 : 4;
+      const char* at = (const char*)a.bias + ((long)w.e * a.N + w.n0) * size;
+      const i32x4 r = make_rsrc(at, w.e == a.E ? 0 : min(a.N - w.n0, BN) * size);
+      lds_load16(r, lane * 16, bias0 + (turn & 3) * (BN * 4));
+    }
+  };
+
+  f32x4 acc[8][8], dbacc[4];
+  auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+        pin_acc(acc[i][j]);
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      dbacc[j] = {0.f, 0.f, 0.f, 0.f};
+      if (KIND == R_TN) pin_vgpr(dbacc[j]);
+    }
+    settle();
+  };
+
+  // P's fragment i, lane l15 of KC: row 128 wn + 32 (i / 2) + 8 (l15 / 4) + 4 (i % 2) + l15 % 4,
+  // so that a lane's results of fragments 2i, 2i + 1 are 8 neighbours, and 32 with the lanes g.
+  // Q's fragment j: rows 32 j + 16 wm + l15, so that both halves of the waves have work in a
+  // tile of few rows. The lanes' addresses are kept, and move between the two places by one
+  // addition a stage: KC has one for each contraction half, KS one for each column base.
+  const unsigned smem0 = lds_addr(smem);
+  constexpr int PA = P_KC ? 2 : 8, QA = Q_KC ? 2 : 4;
+  unsigned pa[PA], qa[QA];
+#pragma unroll
+  for (int x = 0; x < PA; ++x) {
+    if (P_KC) {
+      const int r = wn * 128 + (l15 >> 2) * 8 + (l15 & 3);
+      pa[x] = smem0 + (r * 64 + ((x * 4 + g) ^ kc_swz<3>(r)) * 8) * 2;
+    } else {
+      const int r = g * 8 + (l15 >> 2), col = wn * 128 + x * 16 + 4 * (l15 & 3);
+      pa[x] = smem0 + (r * BN + ((col >> 3) ^ ks_swz(r)) * 8 + (col & 7)) * 2;
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < QA; ++x) {
+    if (Q_KC) {
+      const int r = wm * 16 + l15;
+      qa[x] = smem0 + BSLOT * 2 + (r * 64 + ((x * 4 + g) ^ kc_swz<2>(r)) * 8) * 2;
+    } else {
+      const int r = g * 8 + (l15 >> 2), col = x * 32 + wm * 16 + 4 * (l15 & 3);
+      qa[x] = smem0 + BSLOT * 2 + (r * 128 + ((col >> 3) ^ ks_swz(r)) * 8 + (col & 7)) * 2;
+    }
+  }
+  auto read_p = [&](int kk, int i) {
+    if (P_KC) return lds_read16(pa[kk], ((i >> 1) * 32 + (i & 1) * 4) * 128);
+    return lds_read_tr(pa[i % PA], kk * 32 * BN * 2, 4 * BN * 2);
+  };
+  auto read_q = [&](int kk, int j) {
+    if (Q_KC) return lds_read16(qa[kk], j * 32 * 128);
+    return lds_read_tr(qa[j % QA], (j / 4) * BSLOT + kk * 32 * 128 * 2, 4 * 128 * 2);
+  };
+  int hop = 2 * BSLOT * 2, load_hop = hop;
+  auto other_place = [&]() {
+#pragma unroll
+    for (int x = 0; x < PA; ++x) pa[x] += hop;
+#pragma unroll
+    for (int x = 0; x < QA; ++x) qa[x] += hop;
+    hop = -hop;
+  };
+
+  // ---- epilogue: lane (l15, g) holds rows 32 j + 16 wm + l15 of Q. Every lane stores
+  // every time, to a place past the descriptor's end where it has nothing: the wait
+  // counts on STORES of them.
+  constexpr bool F32 = KIND == R_TN && EPI != R_BF16;
+  constexpr int STORES = F32 || (KIND == R_NT && EPI == R_GELU_DER) ? 52 : 32;  // of 64: the counter goes to 63
+  auto finish = [&](const BigTile& w, int turn) {
+    int l15 = lane & 15, g = lane >> 4;
+    asm volatile("" : "+v"(l15), "+v"(g));  // offsets made from these are not kept through the loop
+    settle();
+    const long base = (KIND == R_TN ? (long)w.e * a.M + w.m0 : w.row0) * a.N + w.n0;
+    const auto rc = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + base * (F32 ? 4 : 2), (short)0, 0x7fffffff, 0x00027000);
+    const auto rd = __builtin_amdgcn_make_buffer_rsrc((char*)a.der + base * 2, (short)0, 0x7fffffff, 0x00027000);
+    const int ncols = a.N - w.n0, nrows = KIND == R_TN ? a.M - w.m0 : w.rows;
+    float bias[KIND == R_NT ? 32 : 1];
+    if (KIND == R_NT) {
+#pragma unroll
+      for (int x = 0; x < 32; ++x) {
+        const int n = wn * 128 + x / 8 * 32 + g * 8 + x % 8;
+        bias[x] = a.bias == nullptr ? 0.f
+                  : a.bias_bf16     ? bf2f(((const __bf16*)bias_lds[turn & 3])[n])
+                                    : bias_lds[turn & 3][n];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pin_acc(acc[i][j]);
+      const int r = j * 32 + wm * 16 + l15;
+      if (F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int n = wn * 128 + i * 16 + g * 4;
+          const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 4 : OOB_OFFSET;
+          f32x4 v = acc[i][j];
+          if (EPI == R_F32_ACC) v += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, off, 0, 0));
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rc, off, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int ip = 0; ip < 4; ++ip) {
+          float v[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) v[x] = acc[2 * ip + x / 4][j][x & 3];
+          int n;
+          if (P_KC) {
+            n = wn * 128 + ip * 32 + g * 8;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] += bias[ip * 8 + x];
+          } else {
+            // fragment 2 ip's columns 4g.. and 2 ip + 1's: lanes of odd g give the first and get the
+            // second, so that each has 8 neighbours
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[x]), __float_as_uint(v[4 + x]),
+                                                              false, false);
+              v[x] = __uint_as_float(s[0]);
+              v[4 + x] = __uint_as_float(s[1]);
+            }
+            n = wn * 128 + (2 * ip + (g & 1)) * 16 + (g >> 1) * 8;
+          }
+          const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
+          bf16x8 o, d;
+          if (KIND == R_NN && EPI == R_MUL)
+            d = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rd, off, 0, 0));
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            if (KIND == R_NT && EPI == R_GELU) {
+              o[x] = f2bf(gelu_of(v[x]));
+            } else if (KIND == R_NT && EPI == R_GELU_DER) {
+              float y, s;
+              gelu_and_slope(v[x], &y, &s);
+              o[x] = f2bf(y);
+              d[x] = f2bf(s);  // the slope, in the outputs' type: one rounding of dP more
+            } else if (KIND == R_NN && EPI == R_MUL) {
+              o[x] = f2bf(v[x] * bf2f(d[x]));
+            } else {
+              o[x] = f2bf(v[x]);
+            }
+          }
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rc, off, 0, 0);
+          if (KIND == R_NT && EPI == R_GELU_DER)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, d), rd, off, 0, 0);
+        }
+      }
+    }
+    if (KIND == R_TN && a.db != nullptr && w.n0 == 0 && g == 0) {  // all 16 D rows hold the same sums
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        pin_vgpr(dbacc[x]);
+        const int m = w.m0 + (4 * wn + x) * 32 + wm * 16 + l15;
+        if (m < a.M) {
+          const long at = (long)w.e * a.M + m;
+          if (a.bias_bf16) ((__bf16*)a.db)[at] = f2bf(dbacc[x][0]);
+          else ((float*)a.db)[at] = (EPI == R_F32_ACC ? ((float*)a.db)[at] : 0.f) + dbacc[x][0];
+        }
+      }
+    }
+  };
+
+  if (mine >= tiles) return;
+  int loading = mine, lt = 0, lturn = 0;  // the tile and stage that are loaded next
+  BigTile lw = decode(loading), w = lw;
+  // past the last tile, nothing is loaded
+  auto next_stage = [&]() {
+    to += load_hop;
+    load_hop = -load_hop;
+    if (loading >= tiles) {
+      pbytes = qbytes = 0;
+      return;
+    }
+    if (++lt < lw.steps) {
+      point_on(lw);
+    } else {
+      lt = 0;
+      ++lturn;
+      loading += stride;
+      if (loading < tiles) {
+        lw = decode(loading);
+        point_at(lw);
+        stage_bias(lw, lturn);
+      } else {
+        pbytes = qbytes = 0;
+      }
+    }
+  };
+
+  bf16x8 p0[8], q0[8], p1[8], q1[8], ones;
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = (__bf16)1.0f;
-
-  // Fragment f, index i of P is tile row p_row: a lane's results in D rows
-  // 4g..4g+3 of all FN fragments are then FN*4 neighbouring outputs (KC only).
-  auto p_row = [&](int f) { return wn * FN * 16 + (l15 >> 2) * (FN * 4) + f * 4 + (l15 & 3); };
-
-  auto read_ks = [&](const __bf16* tile, int cols, int base) {
-    // lane i of 16 gets column base + i at 4 rows; lanes' addresses: row i >> 2, columns 4 (i & 3)
-    const int r = g * 8 + (l15 >> 2), col = base + 4 * (l15 & 3);
-    const int c0 = ((col >> 3) ^ ks_swz(r)) * 8 + (col & 7);
-    const int c1 = ((col >> 3) ^ ks_swz(r + 4)) * 8 + (col & 7);
-    bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, tile + r * cols + c0));
-    bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, tile + (r + 4) * cols + c1));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  asm volatile("" : "+v"(ones));  // not made anew before each product
+  // A quarter of a stage: 32 MFMAs, with `gap(x)`, x = 0 .. 15, behind every other. Those
+  // of the second rows (j0 = 4) are left out where a tile has none.
+  auto quarter = [&](const bf16x8(&p)[8], const bf16x8(&q)[8], auto j0_, bool there, bool with_db, auto gap) {
+    constexpr int j0 = decltype(j0_)::value;
+    if (j0 == 0 || there) {
+      each16([&](auto x) {
+        constexpr int X = decltype(x)::value, j = j0 + X / 4, i = X % 4 * 2;
+        mfma_acc(acc[i][j], p[i], q[j]);
+        mfma_acc(acc[i + 1][j], p[i + 1], q[j]);
+        __builtin_amdgcn_sched_barrier(0);
+        gap(x);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if (KIND == R_TN && with_db && wn == j0 / 4) {  // db: the sums of Q's columns
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mfma_vgpr(dbacc[j], ones, q[j0 + j]);
+      }
+    } else {
+      each16(gap);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const std::integral_constant<int, 0> first_rows;
+  const std::integral_constant<int, 4> last_rows;
+  auto load = [&](auto x) {
+    constexpr int X = decltype(x)::value;
+    if constexpr (X < 8) load_p(x);
+    else load_q(std::integral_constant<int, X - 8>());
+  };
+  auto read0 = [&](auto x) {
+    constexpr int X = decltype(x)::value;
+    if constexpr (X < 8) p0[X] = read_p(0, X);
+    else q0[X - 8] = read_q(0, X - 8);
+  };
+  auto read1 = [&](auto x) {
+    constexpr int X = decltype(x)::value;
+    if constexpr (X < 8) p1[X] = read_p(1, X);
+    else q1[X - 8] = read_q(1, X - 8);
   };
 
-  for (int t = 0; t < STAGES - 1 && t < steps; ++t) stage(t, t);
-  int buf = 0;
-  for (int t = 0; t < steps; ++t) {
-    // stage t has landed; every wave is past its reads of stage t - 1, whose place is refilled
-    if (t + STAGES - 2 < steps) wait_and_barrier<(STAGES - 2) * (PL + QL)>();
-    else wait_and_barrier<0>();
-    if (t + STAGES - 1 < steps) stage(t + STAGES - 1, buf == 0 ? STAGES - 1 : buf - 1);
-    const __bf16* tp = smem + buf * STAGE;
-    const __bf16* tq = tp + BN * RBK;
-    bf16x8 pf[FN], qf[FM];
+  if (tiles >= 8 * stride)  // XCDs an eighth of a tile apart, so that their stores do not come all at once
+    for (int i = (blockIdx.x & 7) * w.steps; i > 0; --i) __builtin_amdgcn_s_sleep(5);
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      if (Q_KC) {
-        const int r = wm * FM * 16 + j * 16 + l15;
-        qf[j] = *(const bf16x8*)(tq + r * RBK + (g ^ kc_swz<2>(r)) * 8);
-      } else {
-        qf[j] = read_ks(tq, BM, wm * FM * 16 + j * 16);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < FN; ++i) {
-      if (P_KC) {
-        const int r = p_row(i);
-        pf[i] = *(const bf16x8*)(tp + r * RBK + (g ^ kc_swz<PSHIFT>(r)) * 8);
-      } else {
-        pf[i] = read_ks(tp, BN, wn * FN * 16 + i * 16);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-      for (int j = 0; j < FM; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pf[i], qf[j], acc[i][j], 0, 0, 0);
-    if (KIND == R_TN && with_db) {
-#pragma unroll
-      for (int j = 0; j < FM; ++j)
-        dbacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, qf[j], dbacc[j], 0, 0, 0);
-    }
-    buf = buf == STAGES - 1 ? 0 : buf + 1;
+  for (int i = 0; i < 8; ++i) {
+    pv[i] = pv0[i];
+    qv[i] = qv0[i];
   }
-
-  // ---- epilogue: lane (l15, g) holds output row 16j + l15
-#pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    const int r = wm * FM * 16 + j * 16 + l15;
-    if (KIND == R_TN) {
-      if (m0 + r < a.M) {
-        const long at = ((long)e * a.M + m0 + r) * a.N;
-#pragma unroll
-        for (int i = 0; i < FN; ++i) {
-          const int n = n0 + wn * FN * 16 + i * 16 + g * 4;
-          if (n < a.N) {
-            if (EPI == R_BF16) {
-              bf16x4 o;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) o[q] = f2bf(acc[i][j][q]);
-              *(bf16x4*)((__bf16*)a.C + at + n) = o;
-            } else {
-              float* c = (float*)a.C + at + n;
-              *(f32x4*)c = EPI == R_F32_ACC ? *(const f32x4*)c + acc[i][j] : acc[i][j];
-            }
-          }
+  stage_bias(lw, 0);
+  point_at(lw);
+  each16(load);
+  next_stage();
+  each16(load);
+  wait_and_barrier<16>();
+  each16(read0);
+  next_stage();
+  bool stored = false;  // the last tile's stores lie between this stage and the one before
+  for (int at = mine, turn = 0; at < tiles; at += stride, ++turn) {
+    if (turn > 0) w = decode(at);
+    const bool both = KIND == R_TN || w.rows > 128;  // the tile's second half of rows is there
+    const bool with_db = KIND == R_TN && a.db != nullptr && w.n0 == 0;
+    clear();
+    for (int t = 0; t < w.steps; ++t) {
+      quarter(p0, q0, first_rows, true, with_db, [&](auto x) {
+        constexpr int X = decltype(x)::value;  // the last of them early enough to be there at the barrier
+        if constexpr (X < 4) {
+          read1(std::integral_constant<int, 2 * X>());
+          read1(std::integral_constant<int, 2 * X + 1>());
+        } else if constexpr (X < 12) {
+          read1(std::integral_constant<int, X + 4>());
         }
-        if (with_db && g == 0) {  // all 16 D rows hold the same sums
-          const long at_b = (long)e * a.M + m0 + r;
-          if (a.bias_bf16) ((__bf16*)a.db)[at_b] = f2bf(dbacc[j][0]);
-          else ((float*)a.db)[at_b] = (EPI == R_F32_ACC ? ((float*)a.db)[at_b] : 0.f) + dbacc[j][0];
-        }
-      }
-    } else if (r < rows) {
-      const long at = (row0 + r) * a.N;
-      constexpr int STEP = P_KC ? 8 : 4;  // neighbouring outputs stored at once
-#pragma unroll
-      for (int i0 = 0; i0 < FN; i0 += STEP / 4) {
-        const int n = n0 + wn * FN * 16 + (P_KC ? g * (FN * 4) + i0 * 4 : i0 * 16 + g * 4);
-        if (n < a.N) {
-          float v[STEP];
-#pragma unroll
-          for (int q = 0; q < STEP; ++q) v[q] = acc[i0 + q / 4][j][q & 3];
-          if (KIND == R_NT && a.bias != nullptr && e < a.E) {
-            if (a.bias_bf16) {
-              const bf16x8 b = *(const bf16x8*)((const __bf16*)a.bias + (long)e * a.N + n);
-#pragma unroll
-              for (int q = 0; q < STEP; ++q) v[q] += bf2f(b[q & 7]);
-            } else {
-#pragma unroll
-              for (int h = 0; h < STEP; h += 4) {
-                const f32x4 b = *(const f32x4*)((const float*)a.bias + (long)e * a.N + n + h);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) v[h + q] += b[q];
-              }
-            }
-          }
-          typedef __attribute__((ext_vector_type(STEP))) __bf16 outv;
-          outv o, d;
-          if (EPI == R_MUL) d = *(const outv*)(a.der + at + n);
-#pragma unroll
-          for (int q = 0; q < STEP; ++q) {
-            if (EPI == R_GELU) {
-              o[q] = f2bf(gelu_of(v[q]));
-            } else if (EPI == R_GELU_DER) {
-              float y, s;
-              gelu_and_slope(v[q], &y, &s);
-              o[q] = f2bf(y);
-              d[q] = f2bf(s);  // the slope, in the outputs' type: one rounding of dP more
-            } else if (EPI == R_MUL) {
-              o[q] = f2bf(v[q] * bf2f(d[q]));
-            } else {
-              o[q] = f2bf(v[q]);
-            }
-          }
-          *(outv*)((__bf16*)a.C + at + n) = o;
-          if (EPI == R_GELU_DER) *(outv*)(a.der + at + n) = d;
-        }
-      }
+      });
+      wait_reads_and_barrier();  // nobody reads this stage any more
+      // A CU takes 64 bytes a cycle: a stage's loads keep it busy for half a stage, and
+      // where they come faster the wave stands at the next one and multiplies nothing.
+      quarter(p0, q0, last_rows, both, with_db, [&](auto x) {
+        constexpr int X = decltype(x)::value;
+        if constexpr (X % 3 == 0 && X < 15) load(std::integral_constant<int, X / 3>());
+      });
+      other_place();
+      quarter(p1, q1, first_rows, true, with_db, [&](auto x) {
+        constexpr int X = decltype(x)::value;
+        if constexpr (X % 3 == 0) load(std::integral_constant<int, 5 + X / 3>());
+      });
+      // the next stage has landed
+      if (stored) wait_and_barrier<11 + STORES>();
+      else wait_and_barrier<11>();
+      stored = false;
+      quarter(p1, q1, last_rows, both, with_db, [&](auto x) {
+        constexpr int X = decltype(x)::value;
+        read0(x);
+        if constexpr (X % 3 == 1 && X < 15) load(std::integral_constant<int, 11 + X / 3>());
+        if constexpr (X == 15) next_stage();
+      });
     }
+    finish(w, turn);
+    stored = true;
   }
+  // nothing may come into this block's LDS once it is another's
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
 
 template <int KIND, int EPI>
-static void launch_ragged(const RaggedArgs& a, hipStream_t stream) {
-  constexpr int WN = 2, WM = 2, FN = 8, FM = 4, BN = WN * FN * 16, BM = WM * FM * 16;
-  const long nt = (a.N + BN - 1) / BN;
-  const long tiles = KIND == R_TN ? (long)a.E * ((a.M + BM - 1) / BM) * nt
-                                  : (a.R / BM + a.E + 1) * nt;
-  hipLaunchKernelGGL((ragged_gemm_kernel<KIND, EPI, WN, WM, FN, FM, 3>), dim3((unsigned)tiles),
-                     dim3(WN * WM * 64), 0, stream, a);
+static void launch_rows(const RaggedArgs& a, void* table, hipStream_t stream) {
+  if (table != nullptr) {
+    hipLaunchKernelGGL(ragged_tiles_kernel, dim3(1), dim3(1024), 0, stream, a.offsets, a.E, a.R, (int4*)table);
+    const long most = (a.R / BM + a.E + 1) * ((a.N + BN - 1) / BN);
+    hipLaunchKernelGGL((ragged_big_kernel<KIND, EPI>), dim3((unsigned)(most < 256 ? most : 256)), dim3(BT), 0,
+                       stream, a, (const int4*)table);
+    return;
+  }
+  const long tiles = (a.R / RBM + a.E + 1) * ((a.N + RBN - 1) / RBN);
+  hipLaunchKernelGGL((ragged_rows_kernel<KIND, EPI>), dim3((unsigned)tiles), dim3(RT), 0, stream, a);
 }
 
+template <int OUT>
+static void launch_weights(const RaggedArgs& a, hipStream_t stream) {
+  const long tiles = (long)a.E * ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
+  hipLaunchKernelGGL((ragged_big_kernel<R_TN, OUT>), dim3((unsigned)(tiles < 256 ? tiles : 256)), dim3(BT), 0,
+                     stream, a, (const int4*)nullptr);
+}
+
+// int4 entries a table of M-tiles needs
+extern "C" long lah_ragged_tiles_room(long R, int E) { return R / BM + E + 2; }
+
+// table: room for the M-tiles where the large tiles are to be used, or null
 extern "C" void lah_ragged_nt(const void* x, const void* w, void* y, const void* offsets,
                               const void* bias, int bias_bf16, void* der, long R, int E, int N,
-                              int K, int epi, hipStream_t stream) {
+                              int K, int epi, void* table, hipStream_t stream) {
   RaggedArgs a{(const __bf16*)w, (const __bf16*)x, y, (const int*)offsets, bias, (__bf16*)der,
                nullptr, R, E, N, 0, K, bias_bf16};
-  if (epi == R_GELU_DER) launch_ragged<R_NT, R_GELU_DER>(a, stream);
-  else if (epi == R_GELU) launch_ragged<R_NT, R_GELU>(a, stream);
-  else launch_ragged<R_NT, R_PLAIN>(a, stream);
+  if (epi == R_GELU_DER) launch_rows<R_NT, R_GELU_DER>(a, table, stream);
+  else if (epi == R_GELU) launch_rows<R_NT, R_GELU>(a, table, stream);
+  else launch_rows<R_NT, R_PLAIN>(a, table, stream);
 }
 
 // dx[r] = W[e]^T d[r] (times der[r], if given): W [E, K, N], d [R, K], out [R, N]
 extern "C" void lah_ragged_nn(const void* d, const void* w, void* out, const void* offsets,
-                              void* der, long R, int E, int N, int K, hipStream_t stream) {
+                              void* der, long R, int E, int N, int K, void* table,
+                              hipStream_t stream) {
   RaggedArgs a{(const __bf16*)w, (const __bf16*)d, out, (const int*)offsets, nullptr,
                (__bf16*)der, nullptr, R, E, N, 0, K, 0};
-  if (der != nullptr) launch_ragged<R_NN, R_MUL>(a, stream);
-  else launch_ragged<R_NN, R_PLAIN>(a, stream);
+  if (der != nullptr) launch_rows<R_NN, R_MUL>(a, table, stream);
+  else launch_rows<R_NN, R_PLAIN>(a, table, stream);
 }
 
 // dw[e] = sum_r d[r] x[r]^T: d [R, M], x [R, N], dw [E, M, N]; db [E, M] or null
@@ -422,7 +976,7 @@ extern "C" void lah_ragged_tn(const void* d, const void* x, void* dw, void* db, 
                               hipStream_t stream) {
   RaggedArgs a{(const __bf16*)x, (const __bf16*)d, dw, (const int*)offsets, nullptr, nullptr,
                db, R, E, N, M, 0, db_bf16};
-  if (out == R_BF16) launch_ragged<R_TN, R_BF16>(a, stream);
-  else if (out == R_F32_ACC) launch_ragged<R_TN, R_F32_ACC>(a, stream);
-  else launch_ragged<R_TN, R_F32>(a, stream);
+  if (out == R_BF16) launch_weights<R_BF16>(a, stream);
+  else if (out == R_F32_ACC) launch_weights<R_F32_ACC>(a, stream);
+  else launch_weights<R_F32>(a, stream);
 }
