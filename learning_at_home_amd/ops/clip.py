@@ -15,8 +15,6 @@ import torch
 
 from . import _C, HAS_HIP
 
-_KERNEL_TYPES = (torch.bfloat16, torch.float16, torch.float32)
-
 
 def _listed(tensors) -> list:
     if isinstance(tensors, torch.Tensor):
@@ -24,14 +22,7 @@ def _listed(tensors) -> list:
     tensors = list(tensors)
     if not tensors:
         raise ValueError("no tensors")
-    if any(t.device != tensors[0].device for t in tensors):
-        raise ValueError("all tensors must be on one device")
     return tensors
-
-
-def _kernels_take(tensors) -> bool:
-    return (HAS_HIP and tensors[0].is_cuda
-            and all(t.dtype in _KERNEL_TYPES and t.is_contiguous() for t in tensors))
 
 
 @torch.no_grad()
@@ -44,10 +35,12 @@ def grad_clip_scale(tensors: Sequence[torch.Tensor], max_norm: float,
     tensors = _listed(tensors)
     if not max_norm > 0:
         raise ValueError(f"max_norm must be positive, got {max_norm}")
-    if tensors[0].is_cuda and HAS_HIP:
-        tensors = [t.contiguous() for t in tensors]
-        if _kernels_take(tensors):
-            return tuple(_C.grad_norm(tensors, max_norm, eps))
+    if HAS_HIP and tensors[0].is_cuda:
+        got = _C.grad_norm(tensors, max_norm, eps) or _C.grad_norm([t.contiguous() for t in tensors], max_norm, eps)
+        if got:
+            return tuple(got)
+    if any(t.device != tensors[0].device for t in tensors):
+        raise ValueError("all tensors must be on one device")
     norm = torch.stack([t.float().square().sum(dtype=torch.float64) for t in tensors]).sum().sqrt()
     return norm.float(), (max_norm / (norm + eps)).clamp(max=1.0).float()
 
@@ -59,11 +52,9 @@ def clip_grad_norm_(tensors: Sequence[torch.Tensor], max_norm: float,
     returns the norm they had, on their device."""
     tensors = _listed(tensors)
     norm, scale = grad_clip_scale(tensors, max_norm, eps)
-    if _kernels_take(tensors):
-        _C.grad_scale_(tensors, scale)
-    else:
+    if not (HAS_HIP and tensors[0].is_cuda and _C.grad_scale_(tensors, scale)):
         for t in tensors:
-            t.mul_(scale.to(t.dtype) if t.dtype == torch.float64 else scale)
+            t.mul_(scale)
     return norm
 
 
@@ -85,33 +76,28 @@ def master_sgd_step_(params: Sequence[torch.Tensor], masters: Sequence[torch.Ten
         raise ValueError("params, masters, grads and momentum_bufs must go together")
     if momentum and not bufs:
         raise ValueError("momentum needs momentum_bufs")
+    if not params:
+        return
+    if any(m.dtype != torch.float32 for m in masters + bufs):
+        raise ValueError("masters and momentum_bufs must be fp32")
     if any(p.shape != m.shape or p.shape != g.shape for p, m, g in zip(params, masters, grads)):
         raise ValueError("params, masters and grads must have the same shapes")
     if any(p.shape != b.shape for p, b in zip(params, bufs)):
         raise ValueError("momentum_bufs must have the shapes of the params")
-    if any(m.dtype != torch.float32 for m in masters + bufs):
-        raise ValueError("masters and momentum_bufs must be fp32")
-    if not params:
-        return
-    fits = [HAS_HIP and p.is_cuda and p.dtype == torch.bfloat16 and g.dtype in _KERNEL_TYPES
-            and p.is_contiguous() and m.is_contiguous() and g.is_contiguous()
-            for p, m, g in zip(params, masters, grads)]
-    if bufs:
-        fits = [f and b.is_contiguous() for f, b in zip(fits, bufs)]
-    if all(fits):
-        _C.master_sgd_(params, masters, grads, bufs, grad_scale, lr, momentum, weight_decay)
-        return
-    some = [i for i, f in enumerate(fits) if f]
-    if some:
-        _C.master_sgd_(*([t[i] for i in some] for t in (params, masters, grads)),
-                       [bufs[i] for i in some] if bufs else [], grad_scale, lr, momentum, weight_decay)
-    for i in (i for i, f in enumerate(fits) if not f):
+    if HAS_HIP and params[0].is_cuda:
+        if _C.master_sgd_(params, masters, grads, bufs, grad_scale, lr, momentum, weight_decay):
+            return
+    for i in range(len(params)):
+        b = bufs[i : i + 1]
+        if HAS_HIP and params[i].is_cuda and _C.master_sgd_(params[i : i + 1], masters[i : i + 1], grads[i : i + 1],
+                                                           b, grad_scale, lr, momentum, weight_decay):
+            continue
         u = grads[i].float()
         if grad_scale is not None:
             u = u * grad_scale
         if weight_decay:
             u = u + weight_decay * masters[i]
-        if bufs:
-            u = bufs[i].mul_(momentum).add_(u)
+        if b:
+            u = b[0].mul_(momentum).add_(u)
         masters[i].add_(u, alpha=-lr)
         params[i].copy_(masters[i])

@@ -48,8 +48,10 @@ void lah_ragged_nt(const void*, const void*, void*, const void*, const void*, in
                    long, int, int, int, int, void*, hipStream_t);
 void lah_ragged_nn(const void*, const void*, void*, const void*, void*, long, int, int, int,
                    void*, hipStream_t);
+int lah_ragged_splits(long, int, int, int);
 void lah_ragged_tn(const void*, const void*, void*, void*, int, const void*, long, int, int,
-                   int, int, hipStream_t);
+                   int, int, int, void*, hipStream_t);
+void lah_ragged_slope(const void*, const void*, void*, long, hipStream_t);
 long lah_clip_partials(int);
 void lah_grad_norm(void* const*, const long*, const int*, int, void*, float, float, void*,
                    void*, hipStream_t);
@@ -395,6 +397,11 @@ static void check_ragged(const torch::Tensor& a, const torch::Tensor& b,
   TORCH_CHECK(a.dim() == 2 && a.size(0) < (int64_t)1 << 31, "rows must be [R, K], R < 2^31");
 }
 
+static void check_slope(const torch::Tensor& der) {
+  TORCH_CHECK(der.scalar_type() == at::kHalf, "der must be fp16");
+  CHECK_CONTIG(der); CHECK_ALIGNED(der);
+}
+
 static void check_weight(const torch::Tensor& w, const torch::Tensor& offsets) {
   TORCH_CHECK(w.dim() == 3 && w.size(0) == offsets.numel() - 1, "weight must be [E, N, K]");
   TORCH_CHECK(w.size(1) > 0 && w.size(2) > 0 && w.size(1) % 8 == 0 && w.size(2) % 8 == 0,
@@ -404,10 +411,12 @@ static void check_weight(const torch::Tensor& w, const torch::Tensor& offsets) {
 }
 
 std::vector<torch::Tensor> ragged_layout(torch::Tensor ids, int64_t E) {
-  CHECK_CUDA(ids); CHECK_CONTIG(ids);
+  CHECK_CUDA(ids);
   const bool wide = ids.scalar_type() == at::kLong;
-  TORCH_CHECK(wide || ids.scalar_type() == at::kInt, "ids must be int32 or int64");
-  TORCH_CHECK(E >= 1 && E <= 4096, "1 to 4096 experts, got ", E);
+  TORCH_CHECK_VALUE(ids.dim() == 2 && (wide || ids.scalar_type() == at::kInt),
+                    "topk_idx must be [T, k] int32 or int64, got ", ids.sizes(), " ", ids.scalar_type());
+  TORCH_CHECK_VALUE(E >= 1 && E <= 4096, "1 to 4096 experts, got ", E);
+  ids = ids.contiguous();
   const int64_t n = ids.numel();
   TORCH_CHECK(n < ((int64_t)1 << 31) - 65536, "too many slots");
   ON_DEVICE_OF(ids);
@@ -457,7 +466,7 @@ torch::Tensor ragged_nt(torch::Tensor x, torch::Tensor w, torch::Tensor offsets,
   }
   void* der_p = nullptr;
   if (der.has_value()) {
-    CHECK_BF16(*der); CHECK_CONTIG(*der); CHECK_ALIGNED(*der);
+    check_slope(*der);
     TORCH_CHECK(der->dim() == 2 && der->size(0) == R && der->size(1) == N &&
                 der->device() == x.device(), "der must be [R, N] on the GPU of x");
     der_p = der->data_ptr();
@@ -481,7 +490,7 @@ torch::Tensor ragged_nn(torch::Tensor d, torch::Tensor w, torch::Tensor offsets,
   TORCH_CHECK(d.size(1) == K, "d must be [R, ", K, "], got [", R, ", ", d.size(1), "]");
   void* der_p = nullptr;
   if (der.has_value()) {
-    CHECK_BF16(*der); CHECK_CONTIG(*der); CHECK_ALIGNED(*der);
+    check_slope(*der);
     TORCH_CHECK(der->dim() == 2 && der->size(0) == R && der->size(1) == N &&
                 der->device() == d.device(), "der must be [R, N] on the GPU of d");
     der_p = der->data_ptr();
@@ -522,20 +531,115 @@ void ragged_tn(torch::Tensor d, torch::Tensor x, torch::Tensor offsets, torch::T
     db_p = db->data_ptr();
   }
   ON_DEVICE_OF(d);
+  const int splits = lah_ragged_splits(R, (int)E, (int)N, (int)M);
+  torch::Tensor part;
+  if (splits > 1) part = torch::empty({splits * E * M * (N + 1)}, d.options().dtype(at::kFloat));
   lah_ragged_tn(d.data_ptr(), x.data_ptr(), dw.data_ptr(), db_p, db_bf16, offsets.data_ptr(), R,
-                (int)E, (int)N, (int)M, bf16 ? 2 : accumulate ? 1 : 0,
+                (int)E, (int)N, (int)M, bf16 ? 2 : accumulate ? 1 : 0, splits, ptr_or_null(part),
                 cur_stream());
   CHECK_LAUNCH();
 }
 
+// dP = dy * der
+torch::Tensor ragged_slope(torch::Tensor dy, torch::Tensor der) {
+  CHECK_CUDA(dy); CHECK_BF16(dy); CHECK_CONTIG(dy); CHECK_ALIGNED(dy);
+  check_slope(der);
+  TORCH_CHECK(dy.sizes() == der.sizes() && dy.device() == der.device() && dy.numel() % 8 == 0,
+              "dy and der must go together");
+  ON_DEVICE_OF(dy);
+  auto dp = torch::empty_like(dy);
+  if (dy.numel() == 0) return dp;
+  lah_ragged_slope(dy.data_ptr(), der.data_ptr(), dp.data_ptr(), dy.numel(), cur_stream());
+  CHECK_LAUNCH();
+  return dp;
+}
+
+// ---- the differentiable product ----
+
+// contiguous, from a multiple of 16 bytes on: what the kernels load
+static torch::Tensor ready(const torch::Tensor& t) {
+  const auto c = t.contiguous();
+  return ((uintptr_t)c.data_ptr() & 15) == 0 ? c : c.clone();
+}
+
+struct GroupedLinear : public torch::autograd::Function<GroupedLinear> {
+  static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& x_in,
+                               const torch::Tensor& w_in, const c10::optional<torch::Tensor>& bias,
+                               const torch::Tensor& offsets, bool gelu) {
+    const auto x = ready(x_in), w = ready(w_in);
+    c10::optional<torch::Tensor> b, der;
+    if (bias.has_value()) b = ready(*bias);
+    if (gelu) der = torch::empty({x.size(0), w.size(1)}, x.options().dtype(at::kHalf));
+    ctx->save_for_backward({x, w, offsets, der.value_or(torch::Tensor())});
+    ctx->saved_data["bias"] = b.has_value() ? (int64_t)b->scalar_type() : (int64_t)-1;
+    return ragged_nt(x, w, offsets, b, der, gelu ? 2 : 0);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "grouped_linear is differentiable once");
+    const auto saved = ctx->get_saved_variables();
+    const auto &x = saved[0], &w = saved[1], &offsets = saved[2], &der = saved[3];
+    const int64_t bias = ctx->saved_data["bias"].toInt();
+    if (!grads[0].defined()) return {{}, {}, {}, {}, {}};
+    auto d = ready(grads[0]);
+    if (der.defined()) d = ragged_slope(d, der);
+    torch::Tensor dx, dw, db;
+    const bool want_w = ctx->needs_input_grad(1), want_b = bias >= 0 && ctx->needs_input_grad(2);
+    if (ctx->needs_input_grad(0)) dx = ragged_nn(d, w, offsets, c10::nullopt);
+    if (want_w || want_b) {
+      dw = torch::empty_like(w);
+      c10::optional<torch::Tensor> b;
+      if (want_b) b = db = torch::empty({w.size(0), w.size(1)}, w.options().dtype((at::ScalarType)bias));
+      ragged_tn(d, x, offsets, dw, b, false);
+      if (!want_w) dw = torch::Tensor();
+    }
+    return {dx, dw, db, {}, {}};
+  }
+};
+
+torch::Tensor grouped_linear(torch::Tensor x, torch::Tensor w, torch::Tensor offsets,
+                             c10::optional<torch::Tensor> bias, c10::optional<std::string> activation) {
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 3 && x.size(1) == w.size(2),
+                    "x must be [R, K] and weight [E, N, K], got ", x.sizes(), " and ", w.sizes());
+  TORCH_CHECK_VALUE(offsets.scalar_type() == at::kInt && offsets.dim() == 1 &&
+                    offsets.size(0) == w.size(0) + 1,
+                    "offsets must be [E + 1] int32, got ", offsets.sizes(), " ", offsets.scalar_type());
+  TORCH_CHECK_VALUE(!activation.has_value() || *activation == "gelu",
+                    "activation must be None or 'gelu', got ", activation.value_or(""));
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 && w.scalar_type() == at::kBFloat16,
+                    "the GPU kernels take bf16, got ", x.scalar_type(), " and ", w.scalar_type());
+  TORCH_CHECK_VALUE(w.numel() > 0, "weight must not be empty, got ", w.sizes());
+  TORCH_CHECK_VALUE(w.size(1) % 8 == 0 && w.size(2) % 8 == 0,
+                    "N and K must be multiples of 8 (16-byte rows), got ", w.sizes());
+  TORCH_CHECK_VALUE(w.device() == x.device() && offsets.device() == x.device() &&
+                    (!bias.has_value() || bias->device() == x.device()),
+                    "x, weight, offsets and bias must be on one device");
+  if (bias.has_value()) {
+    TORCH_CHECK_VALUE(bias->dim() == 2 && bias->size(0) == w.size(0) && bias->size(1) == w.size(1),
+                      "bias must be [E, N], got ", bias->sizes());
+    TORCH_CHECK_VALUE(bias->scalar_type() == at::kBFloat16 || bias->scalar_type() == at::kFloat,
+                      "bias must be bf16 or fp32, got ", bias->scalar_type());
+  }
+  const bool gelu = activation.has_value();
+  const auto at = offsets.contiguous();
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || w.requires_grad() || (bias.has_value() && bias->requires_grad())))
+    return GroupedLinear::apply(x, w, bias, at, gelu);
+  c10::optional<torch::Tensor> b;
+  if (bias.has_value()) b = ready(*bias);
+  return ragged_nt(ready(x), ready(w), at, b, c10::nullopt, gelu ? 1 : 0);
+}
+
 // ---- gradient norm, clipping, clipped step of fp32 masters (clip.hip) ----
 
+// kinds of clip.hip; -1: not the kernels'
 static int clip_kind(const torch::Tensor& t) {
   switch (t.scalar_type()) {
     case at::kBFloat16: return 0;
     case at::kHalf: return 1;
     case at::kFloat: return 2;
-    default: TORCH_CHECK(false, "gradients must be bf16, fp16 or fp32, got ", t.scalar_type());
+    default: return -1;
   }
 }
 
@@ -543,21 +647,24 @@ struct ClipList {
   std::vector<void*> p;
   std::vector<long> n;
   std::vector<int> kind;
+  bool taken = true;  // all on one GPU, of kinds and layouts that the kernels take
   explicit ClipList(const std::vector<torch::Tensor>& ts) {
-    TORCH_CHECK(!ts.empty(), "no tensors");
+    TORCH_CHECK_VALUE(!ts.empty(), "no tensors");
+    p.reserve(ts.size()); n.reserve(ts.size()); kind.reserve(ts.size());
     for (const auto& t : ts) {
-      CHECK_CUDA(t);
-      TORCH_CHECK(t.device() == ts[0].device(), "all tensors must be on one GPU");
-      CHECK_CONTIG(t);
+      const int k = clip_kind(t);
+      taken = taken && t.is_cuda() && t.device() == ts[0].device() && k >= 0 && t.is_contiguous();
       p.push_back(t.data_ptr());
       n.push_back(t.numel());
-      kind.push_back(clip_kind(t));
+      kind.push_back(k);
     }
   }
 };
 
-std::vector<torch::Tensor> grad_norm(std::vector<torch::Tensor> grads, double max_norm, double eps) {
+// (norm, scale); nothing where a tensor is not the kernels'
+std::vector<torch::Tensor> grad_norm(const std::vector<torch::Tensor>& grads, double max_norm, double eps) {
   const ClipList l(grads);
+  if (!l.taken) return {};
   ON_DEVICE_OF(grads[0]);
   const auto opt = grads[0].options();
   auto partial = torch::empty({lah_clip_partials((int)l.p.size())}, opt.dtype(at::kDouble));
@@ -568,37 +675,45 @@ std::vector<torch::Tensor> grad_norm(std::vector<torch::Tensor> grads, double ma
   return {norm, scale};
 }
 
-void grad_scale_(std::vector<torch::Tensor> grads, torch::Tensor scale) {
+// whether it was done
+bool grad_scale_(const std::vector<torch::Tensor>& grads, const torch::Tensor& scale) {
   const ClipList l(grads);
+  if (!l.taken) return false;
   const void* s = scale_ptr(scale, grads[0]);
   ON_DEVICE_OF(grads[0]);
   lah_grad_scale(l.p.data(), l.n.data(), l.kind.data(), (int)l.p.size(), s, cur_stream());
   CHECK_LAUNCH();
+  return true;
 }
 
-void master_sgd_(std::vector<torch::Tensor> params, std::vector<torch::Tensor> masters,
-                 std::vector<torch::Tensor> grads, std::vector<torch::Tensor> bufs,
-                 c10::optional<torch::Tensor> scale, double lr, double mu, double weight_decay) {
+// whether it was done: bf16 params with fp32 masters and buffers, all contiguous
+bool master_sgd_(const std::vector<torch::Tensor>& params, const std::vector<torch::Tensor>& masters,
+                 const std::vector<torch::Tensor>& grads, const std::vector<torch::Tensor>& bufs,
+                 const c10::optional<torch::Tensor>& scale, double lr, double mu, double weight_decay) {
   const ClipList p(params), m(masters), g(grads);
-  TORCH_CHECK(p.n == m.n && p.n == g.n, "params, masters and grads must have the same sizes");
-  TORCH_CHECK(params[0].device() == masters[0].device() && params[0].device() == grads[0].device(),
-              "all tensors must be on one GPU");
+  bool taken = p.taken && m.taken && g.taken;
+  TORCH_CHECK_VALUE(p.n == m.n && p.n == g.n, "params, masters and grads must have the same shapes");
+  TORCH_CHECK_VALUE(params[0].device() == masters[0].device() && params[0].device() == grads[0].device(),
+                    "all tensors must be on one device");
   std::vector<void*> b;
   if (!bufs.empty()) {
     const ClipList l(bufs);
-    TORCH_CHECK(l.n == p.n && bufs[0].device() == params[0].device(),
-                "momentum buffers must have the sizes of the params");
-    for (const int k : l.kind) TORCH_CHECK(k == 2, "momentum buffers must be fp32");
+    TORCH_CHECK_VALUE(l.n == p.n, "momentum_bufs must have the shapes of the params");
+    TORCH_CHECK_VALUE(bufs[0].device() == params[0].device(), "all tensors must be on one device");
+    taken = taken && l.taken;
+    for (const int k : l.kind) taken = taken && k == 2;
     b = l.p;
   }
-  for (const int k : p.kind) TORCH_CHECK(k == 0, "params must be bf16");
-  for (const int k : m.kind) TORCH_CHECK(k == 2, "masters must be fp32");
+  for (const int k : p.kind) taken = taken && k == 0;
+  for (const int k : m.kind) taken = taken && k == 2;
+  if (!taken) return false;
   const void* s = scale_ptr(scale, params[0]);
   ON_DEVICE_OF(params[0]);
   lah_master_sgd(p.p.data(), m.p.data(), g.p.data(), b.empty() ? nullptr : b.data(), p.n.data(),
                  g.kind.data(), (int)p.p.size(), s, (float)lr, (float)mu, (float)weight_decay,
                  cur_stream());
   CHECK_LAUNCH();
+  return true;
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -644,6 +759,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("der") = py::none());
   m.def("ragged_tn", &ragged_tn, py::arg("d"), py::arg("x"), py::arg("offsets"), py::arg("dw"),
         py::arg("db") = py::none(), py::arg("accumulate") = false);
+  m.def("grouped_linear", &grouped_linear, py::arg("x"), py::arg("weight"), py::arg("offsets"),
+        py::arg("bias") = py::none(), py::arg("activation") = py::none());
+  m.def("ragged_slope", &ragged_slope, py::arg("dy"), py::arg("der"));
   m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("max_norm"), py::arg("eps") = 1e-6);
   m.def("grad_scale_", &grad_scale_, py::arg("grads"), py::arg("scale"));
   m.def("master_sgd_", &master_sgd_, py::arg("params"), py::arg("masters"), py::arg("grads"),

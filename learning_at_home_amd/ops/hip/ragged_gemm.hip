@@ -36,6 +36,7 @@ enum { R_F32 = 0, R_F32_ACC = 1, R_BF16 = 2 };                // dW outputs
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 #define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
 
 LAH_DEVINL unsigned lds_addr(const void* p) {
@@ -140,11 +141,12 @@ struct RaggedArgs {
   void* C;
   const int* offsets;
   const void* bias;  // NT: [E, N]; fp32 or bf16
-  __bf16* der;       // NT with slope: out; NN with R_MUL: in
+  _Float16* der;     // gelu's slope, below 1.13: 11 bits where bf16 has 8. NT: out; NN with R_MUL: in
   void* db;          // TN: [E, M] or null; fp32 or bf16
   long R;
   int E, N, M, K;    // K: contraction of NT / NN
   int bias_bf16;     // of bias, or of db
+  int splits;        // TN: parts of each expert's rows, each with sums of its own
 };
 
 // Blocks go to the 8 XCDs in turn: of each 512, the 64 that share one XCD (two a
@@ -349,8 +351,10 @@ __launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
         }
       }
       typedef __attribute__((ext_vector_type(STEP))) __bf16 outv;
-      outv o, d;
-      if (EPI == R_MUL) d = *(const outv*)(a.der + at + n);
+      typedef __attribute__((ext_vector_type(STEP))) _Float16 slopev;
+      outv o;
+      slopev d;
+      if (EPI == R_MUL) d = *(const slopev*)(a.der + at + n);
 #pragma unroll
       for (int x = 0; x < STEP; ++x) {
         if (EPI == R_GELU) {
@@ -359,15 +363,129 @@ __launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
           float y, s;
           gelu_and_slope(v[x], &y, &s);
           o[x] = f2bf(y);
-          d[x] = f2bf(s);  // the slope, in the outputs' type: one rounding of dP more
+          d[x] = (_Float16)s;
         } else if (EPI == R_MUL) {
-          o[x] = f2bf(v[x] * bf2f(d[x]));
+          o[x] = f2bf(v[x] * (float)d[x]);
         } else {
           o[x] = f2bf(v[x]);
         }
       }
       *(outv*)((__bf16*)a.C + at + n) = o;
-      if (EPI == R_GELU_DER) *(outv*)(a.der + at + n) = d;
+      if (EPI == R_GELU_DER) *(slopev*)(a.der + at + n) = d;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows (single decoded tokens): each active expert's weight once through the CUs
+//
+// Bound by HBM, or by latency. A block has 16 outputs of one expert for up to 16 of its
+// rows, its 4 waves a quarter of the contraction each; the weight goes from global memory
+// straight into the matrix instruction's registers, and the four sums meet in LDS. Blocks
+// are counted by non-empty tiles, of which there are at most min(R, R / 16 + E + 1): a
+// grid over all experts' slots would start 4112 blocks to find the 64 that one token
+// needs (34 us, 1024 -> 4096 of 256 experts).
+// ---------------------------------------------------------------------------
+#define FR 16  // rows and outputs of a tile
+
+// The tile'th of the tiles of 16 rows of all groups in order (group E: rows of nobody);
+// -1 past the last. Each lane counts some neighbouring groups.
+LAH_DEVINL int find_tile(const RaggedArgs& a, int tile, long* row0, int* rows) {
+  const int lane = threadIdx.x & 63, per = (a.E + 64) / 64;
+  int mine = 0;
+#pragma unroll 4
+  for (int j = 0; j < per; ++j) {
+    const int e = lane * per + j;
+    if (e <= a.E) {
+      long lo, hi;
+      expert_rows(a, e, &lo, &hi);
+      mine += (int)((hi - lo + FR - 1) / FR);
+    }
+  }
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(upto, d, 64);
+    if (lane >= d) upto += v;
+  }
+  // the lane whose groups hold the tile looks through them again
+  int skip = tile - (upto - mine), found = -1, first = 0, count = 0;
+#pragma unroll 4
+  for (int j = 0; j < per; ++j) {
+    const int e = lane * per + j;
+    if (e <= a.E) {
+      long lo, hi;
+      expert_rows(a, e, &lo, &hi);
+      const int n = (int)((hi - lo + FR - 1) / FR);
+      if (skip >= 0 && skip < n) {
+        found = e;
+        first = (int)(lo + (long)skip * FR);
+        count = (int)min(hi - lo - (long)skip * FR, (long)FR);
+      }
+      skip -= n;
+    }
+  }
+  const unsigned long long has = __ballot(found >= 0);
+  if (has == 0) return -1;
+  const int owner = __builtin_amdgcn_readfirstlane(__ffsll(has) - 1);
+  *row0 = __builtin_amdgcn_readlane(first, owner);
+  *rows = __builtin_amdgcn_readlane(count, owner);
+  return __builtin_amdgcn_readlane(found, owner);
+}
+
+template <int EPI>
+__launch_bounds__(256) __global__ void ragged_few_kernel(RaggedArgs a, int per) {
+  __shared__ __attribute__((aligned(16))) float part[2][4][16][20];  // [wave][row][output]; 20: rows 20 banks apart
+  const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  long row0 = 0;
+  int rows = 0;
+  const int e = find_tile(a, blockIdx.y, &row0, &rows);
+  if (e < 0) return;
+  const bool nobody = e == a.E;
+  const int chunks = cdiv(a.K, 32), c0 = chunks * wave / 4, c1 = chunks * (wave + 1) / 4;
+  const bool row_ok = l15 < rows;
+  const __bf16* x = a.Q + (row0 + (row_ok ? l15 : 0)) * a.K + g * 8;
+  for (int n0 = blockIdx.x * per * FR, i = 0; i < per && n0 < a.N; ++i, n0 += FR) {
+    f32x4 acc[2];
+    acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!nobody) {
+      const __bf16* w = a.P + ((long)e * a.N + min(n0 + l15, a.N - 1)) * a.K + g * 8;
+      int c = c0;
+      for (; c + 8 <= c1 && (c + 8) * 32 <= a.K; c += 8) {
+        bf16x8 wf[8], xf[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) wf[u] = *(const bf16x8*)(w + (c + u) * 32);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) xf[u] = row_ok ? *(const bf16x8*)(x + (c + u) * 32) : bf16x8{};
+#pragma unroll
+        for (int u = 0; u < 8; ++u) acc[u & 1] = MFMA(wf[u], xf[u], acc[u & 1]);
+      }
+      for (; c < c1; ++c) {
+        const bool in = c * 32 + g * 8 < a.K;  // past the contraction's end: zeros
+        const bf16x8 wf = in ? *(const bf16x8*)(w + c * 32) : bf16x8{};
+        const bf16x8 xf = in && row_ok ? *(const bf16x8*)(x + c * 32) : bf16x8{};
+        acc[0] = MFMA(wf, xf, acc[0]);
+      }
+    }
+    float(*sums)[16][20] = part[i & 1];  // the other one is still read
+    *(f32x4*)&sums[wave][l15][g * 4] = acc[0] + acc[1];
+    __syncthreads();
+    const int r = tid >> 4, n = n0 + (tid & 15);  // one output a thread
+    if (r >= rows || n >= a.N) continue;
+    float v = (sums[0][r][tid & 15] + sums[1][r][tid & 15]) + (sums[2][r][tid & 15] + sums[3][r][tid & 15]);
+    if (a.bias != nullptr && !nobody) {
+      const long at = (long)e * a.N + n;
+      v += a.bias_bf16 ? bf2f(((const __bf16*)a.bias)[at]) : ((const float*)a.bias)[at];
+    }
+    const long at = (row0 + r) * a.N + n;
+    if (EPI == R_GELU_DER) {
+      float y, s;
+      gelu_and_slope(v, &y, &s);
+      ((__bf16*)a.C)[at] = f2bf(y);
+      a.der[at] = (_Float16)s;
+    } else {
+      ((__bf16*)a.C)[at] = f2bf(EPI == R_GELU ? gelu_of(v) : v);
     }
   }
 }
@@ -499,7 +617,7 @@ template <typename F>
 LAH_DEVINL void each16(F&& f) { each_of(f, std::make_integer_sequence<int, 16>()); }
 
 struct BigTile {
-  int e, rows, steps, m0, n0;
+  int e, part = 0, rows, steps, m0, n0;
   long row0;
 };
 
@@ -516,7 +634,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   const int NT = cdiv(a.N, BN);
   // M-tiles of one expert, or of all
   const int MT = KIND == R_TN ? cdiv(a.M, BM) : __builtin_amdgcn_readfirstlane(table[0].x);
-  const int tiles = KIND == R_TN ? a.E * MT * NT : MT * NT;
+  const int tiles = KIND == R_TN ? a.splits * a.E * MT * NT : MT * NT;
   // 32 neighbouring tiles at a time on the 32 CUs of an XCD (blocks go to XCDs in turn)
   const int stride = gridDim.x;
   const int mine = stride % 256 == 0 ? (blockIdx.x & ~255) | ((blockIdx.x & 7) << 5) | ((blockIdx.x >> 3) & 31)
@@ -533,10 +651,13 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     const int m = first + in % size;
     w.n0 = in / size * BN;
     if (KIND == R_TN) {
+      w.part = w.e / a.E;
+      w.e -= w.part * a.E;
       long lo, hi;
       expert_rows(a, w.e, &lo, &hi);
-      w.row0 = lo;
-      w.rows = (int)(hi - lo);
+      const long each = a.splits == 1 ? hi - lo : (((hi - lo) / a.splits + 64) & ~63L);
+      w.row0 = min(lo + w.part * each, hi);
+      w.rows = (int)min(each, hi - w.row0);
       w.m0 = m * BM;
       w.steps = max(cdiv(w.rows, 64), 1);
     } else {
@@ -704,7 +825,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     int l15 = lane & 15, g = lane >> 4;
     asm volatile("" : "+v"(l15), "+v"(g));  // offsets made from these are not kept through the loop
     settle();
-    const long base = (KIND == R_TN ? (long)w.e * a.M + w.m0 : w.row0) * a.N + w.n0;
+    const long base = (KIND == R_TN ? ((long)w.part * a.E + w.e) * a.M + w.m0 : w.row0) * a.N + w.n0;
     const auto rc = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + base * (F32 ? 4 : 2), (short)0, 0x7fffffff, 0x00027000);
     const auto rd = __builtin_amdgcn_make_buffer_rsrc((char*)a.der + base * 2, (short)0, 0x7fffffff, 0x00027000);
     const int ncols = a.N - w.n0, nrows = KIND == R_TN ? a.M - w.m0 : w.rows;
@@ -756,9 +877,10 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
             n = wn * 128 + (2 * ip + (g & 1)) * 16 + (g >> 1) * 8;
           }
           const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
-          bf16x8 o, d;
+          bf16x8 o;
+          f16x8 d;
           if (KIND == R_NN && EPI == R_MUL)
-            d = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rd, off, 0, 0));
+            d = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(rd, off, 0, 0));
 #pragma unroll
           for (int x = 0; x < 8; ++x) {
             if (KIND == R_NT && EPI == R_GELU) {
@@ -767,9 +889,9 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
               float y, s;
               gelu_and_slope(v[x], &y, &s);
               o[x] = f2bf(y);
-              d[x] = f2bf(s);  // the slope, in the outputs' type: one rounding of dP more
+              d[x] = (_Float16)s;
             } else if (KIND == R_NN && EPI == R_MUL) {
-              o[x] = f2bf(v[x] * bf2f(d[x]));
+              o[x] = f2bf(v[x] * (float)d[x]);
             } else {
               o[x] = f2bf(v[x]);
             }
@@ -786,7 +908,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
         pin_vgpr(dbacc[x]);
         const int m = w.m0 + (4 * wn + x) * 32 + wm * 16 + l15;
         if (m < a.M) {
-          const long at = (long)w.e * a.M + m;
+          const long at = ((long)w.part * a.E + w.e) * a.M + m;
           if (a.bias_bf16) ((__bf16*)a.db)[at] = f2bf(dbacc[x][0]);
           else ((float*)a.db)[at] = (EPI == R_F32_ACC ? ((float*)a.db)[at] : 0.f) + dbacc[x][0];
         }
@@ -926,8 +1048,25 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
 
+// 16-row tiles where experts have a row or none, or there are few rows at all. Of 256
+// experts, 1024 -> 4096, 4 rows take 12 us so and 49 in 128-row tiles, 128 rows 158 and 168,
+// 1024 rows 422 and 361; of 4 experts 64 rows 15 and 22, 256 rows 41 and 23.
+template <int EPI>
+static bool launch_few(const RaggedArgs& a, hipStream_t stream) {
+  if (a.R > a.E && a.R > 64) return false;
+  const long most = a.R < a.R / FR + a.E + 1 ? a.R : a.R / FR + a.E + 1;
+  const int groups = cdiv(a.N, FR);
+  // outputs a block, one group of 16 after the other: looking up its tile is as long as one
+  const int per = (int)(most * groups <= 8192 ? 1 : most * groups <= 32768 ? 4 : 8);
+  hipLaunchKernelGGL((ragged_few_kernel<EPI>), dim3(cdiv(groups, per), (unsigned)most), dim3(256), 0, stream, a,
+                     per);
+  return true;
+}
+
 template <int KIND, int EPI>
 static void launch_rows(const RaggedArgs& a, void* table, hipStream_t stream) {
+  if constexpr (KIND == R_NT)
+    if (launch_few<EPI>(a, stream)) return;
   if (table != nullptr) {
     hipLaunchKernelGGL(ragged_tiles_kernel, dim3(1), dim3(1024), 0, stream, a.offsets, a.E, a.R, (int4*)table);
     const long most = (a.R / BM + a.E + 1) * ((a.N + BN - 1) / BN);
@@ -939,9 +1078,35 @@ static void launch_rows(const RaggedArgs& a, void* table, hipStream_t stream) {
   hipLaunchKernelGGL((ragged_rows_kernel<KIND, EPI>), dim3((unsigned)tiles), dim3(RT), 0, stream, a);
 }
 
+// dW and db from the parts' sums, in the parts' order
+template <int OUT>
+__launch_bounds__(256) __global__ void ragged_join_kernel(const float* __restrict__ part, int splits, long n,
+                                                          void* __restrict__ out) {
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 sum = *(const f32x4*)(part + i);
+  for (int s = 1; s < splits; ++s) sum += *(const f32x4*)(part + s * n + i);
+  if (OUT == R_BF16) {
+    bf16x4 o;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o[x] = f2bf(sum[x]);
+    *(bf16x4*)((__bf16*)out + i) = o;
+  } else {
+    float* c = (float*)out + i;
+    *(f32x4*)c = OUT == R_F32_ACC ? *(const f32x4*)c + sum : sum;
+  }
+}
+
+static void join(const float* part, int splits, long n, void* out, int kind, hipStream_t stream) {
+  const dim3 grid((unsigned)((n / 4 + 255) / 256)), block(256);
+  if (kind == R_BF16) hipLaunchKernelGGL((ragged_join_kernel<R_BF16>), grid, block, 0, stream, part, splits, n, out);
+  else if (kind == R_F32_ACC) hipLaunchKernelGGL((ragged_join_kernel<R_F32_ACC>), grid, block, 0, stream, part, splits, n, out);
+  else hipLaunchKernelGGL((ragged_join_kernel<R_F32>), grid, block, 0, stream, part, splits, n, out);
+}
+
 template <int OUT>
 static void launch_weights(const RaggedArgs& a, hipStream_t stream) {
-  const long tiles = (long)a.E * ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
+  const long tiles = (long)a.splits * a.E * ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
   hipLaunchKernelGGL((ragged_big_kernel<R_TN, OUT>), dim3((unsigned)(tiles < 256 ? tiles : 256)), dim3(BT), 0,
                      stream, a, (const int4*)nullptr);
 }
@@ -953,8 +1118,8 @@ extern "C" long lah_ragged_tiles_room(long R, int E) { return R / BM + E + 2; }
 extern "C" void lah_ragged_nt(const void* x, const void* w, void* y, const void* offsets,
                               const void* bias, int bias_bf16, void* der, long R, int E, int N,
                               int K, int epi, void* table, hipStream_t stream) {
-  RaggedArgs a{(const __bf16*)w, (const __bf16*)x, y, (const int*)offsets, bias, (__bf16*)der,
-               nullptr, R, E, N, 0, K, bias_bf16};
+  RaggedArgs a{(const __bf16*)w, (const __bf16*)x, y, (const int*)offsets, bias, (_Float16*)der,
+               nullptr, R, E, N, 0, K, bias_bf16, 1};
   if (epi == R_GELU_DER) launch_rows<R_NT, R_GELU_DER>(a, table, stream);
   else if (epi == R_GELU) launch_rows<R_NT, R_GELU>(a, table, stream);
   else launch_rows<R_NT, R_PLAIN>(a, table, stream);
@@ -965,18 +1130,59 @@ extern "C" void lah_ragged_nn(const void* d, const void* w, void* out, const voi
                               void* der, long R, int E, int N, int K, void* table,
                               hipStream_t stream) {
   RaggedArgs a{(const __bf16*)w, (const __bf16*)d, out, (const int*)offsets, nullptr,
-               (__bf16*)der, nullptr, R, E, N, 0, K, 0};
+               (_Float16*)der, nullptr, R, E, N, 0, K, 0, 1};
   if (der != nullptr) launch_rows<R_NN, R_MUL>(a, table, stream);
   else launch_rows<R_NN, R_PLAIN>(a, table, stream);
 }
 
-// dw[e] = sum_r d[r] x[r]^T: d [R, M], x [R, N], dw [E, M, N]; db [E, M] or null
+// Parts of each expert's rows, where there are fewer tiles than CUs and many rows to sum: at
+// least 4 stages a part. 16 experts of 1024 rows, 512 x 512: 93 us in one part.
+extern "C" int lah_ragged_splits(long R, int E, int N, int M) {
+  const long tiles = (long)E * ((M + BM - 1) / BM) * ((N + BN - 1) / BN), most = R / E / 256;
+  const long s = tiles < 256 ? 256 / tiles : 1;
+  return (int)(s < most ? s : most < 1 ? 1 : most);
+}
+
+// dw[e] = sum_r d[r] x[r]^T: d [R, M], x [R, N], dw [E, M, N]; db [E, M] or null;
+// part: fp32 room for splits * E * M * (N + 1), if there are more than one
 extern "C" void lah_ragged_tn(const void* d, const void* x, void* dw, void* db, int db_bf16,
-                              const void* offsets, long R, int E, int N, int M, int out,
-                              hipStream_t stream) {
+                              const void* offsets, long R, int E, int N, int M, int out, int splits,
+                              void* part, hipStream_t stream) {
   RaggedArgs a{(const __bf16*)x, (const __bf16*)d, dw, (const int*)offsets, nullptr, nullptr,
-               db, R, E, N, M, 0, db_bf16};
+               db, R, E, N, M, 0, db_bf16, splits};
+  if (splits > 1) {
+    const long n = (long)E * M * N;
+    float* db_part = (float*)part + splits * n;
+    a.C = part;
+    a.db = db != nullptr ? db_part : nullptr;
+    a.bias_bf16 = 0;
+    launch_weights<R_F32>(a, stream);
+    join((const float*)part, splits, n, dw, out, stream);
+    if (db != nullptr)
+      join(db_part, splits, (long)E * M, db, db_bf16 ? R_BF16 : out == R_F32_ACC ? R_F32_ACC : R_F32, stream);
+    return;
+  }
   if (out == R_BF16) launch_weights<R_BF16>(a, stream);
   else if (out == R_F32_ACC) launch_weights<R_F32_ACC>(a, stream);
   else launch_weights<R_F32>(a, stream);
+}
+
+// dP = dy * slope, rounded to bf16 for the two products that take it
+__launch_bounds__(256) __global__ void ragged_slope_kernel(const __bf16* __restrict__ dy,
+                                                           const _Float16* __restrict__ der,
+                                                           __bf16* __restrict__ dp, long n) {
+  for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long)gridDim.x * 2048) {
+    const bf16x8 y = *(const bf16x8*)(dy + i);
+    const f16x8 d = *(const f16x8*)(der + i);
+    bf16x8 o;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) o[x] = f2bf(bf2f(y[x]) * (float)d[x]);
+    *(bf16x8*)(dp + i) = o;
+  }
+}
+
+extern "C" void lah_ragged_slope(const void* dy, const void* der, void* dp, long n, hipStream_t stream) {
+  const long blocks = (n / 8 + 255) / 256;
+  hipLaunchKernelGGL(ragged_slope_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream,
+                     (const __bf16*)dy, (const _Float16*)der, (__bf16*)dp, n);
 }

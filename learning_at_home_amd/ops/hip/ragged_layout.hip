@@ -84,10 +84,18 @@ void layout_place_kernel(const Id* __restrict__ ids, long n, int E, int bits, co
     if (grp < groups)
       for (int e = tid % Ep; e < E; e += Ep) {
         int before = 0, all = 0;
-        for (int q = grp; q < B; q += groups) {
-          const int c = table[(long)q * E + e];
-          all += c;
-          before += q < b ? c : 0;
+        for (int q0 = grp; q0 < B; q0 += 16 * groups) {  // 16 loads at once
+          int c[16];
+#pragma unroll
+          for (int u = 0; u < 16; ++u) {
+            const int q = q0 + u * groups;
+            c[u] = q < B ? table[(long)q * E + e] : 0;
+          }
+#pragma unroll
+          for (int u = 0; u < 16; ++u) {
+            all += c[u];
+            before += q0 + u * groups < b ? c[u] : 0;
+          }
         }
         atomicAdd(&start[e], before);  // whole numbers: the order does not matter
         atomicAdd(&total[e], all);

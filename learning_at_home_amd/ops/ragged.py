@@ -41,18 +41,17 @@ class RaggedLayout(NamedTuple):
     rows: torch.Tensor
 
 
-@torch.no_grad()
 def ragged_layout(topk_idx: torch.Tensor, num_experts: int) -> RaggedLayout:
     """Rows of each expert from the router's choice topk_idx [T, k] (int32 or
     int64): slots sorted by expert, and by slot within one. Ids outside
     [0, num_experts) choose nobody."""
+    if topk_idx.is_cuda and HAS_HIP:
+        return RaggedLayout(*_C.ragged_layout(topk_idx, num_experts))
     if topk_idx.dim() != 2 or topk_idx.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"topk_idx must be [T, k] int32 or int64, got "
                          f"{tuple(topk_idx.shape)} {topk_idx.dtype}")
     if not 1 <= num_experts <= 4096:
         raise ValueError(f"1 to 4096 experts, got {num_experts}")
-    if topk_idx.is_cuda and HAS_HIP:
-        return RaggedLayout(*_C.ragged_layout(topk_idx.contiguous(), num_experts))
     flat = topk_idx.reshape(-1).long()
     key = torch.where((flat >= 0) & (flat < num_experts), flat, num_experts)
     order = torch.argsort(key, stable=True)
@@ -104,11 +103,7 @@ def _check_product(x, weight, offsets, bias, activation):
         raise ValueError(f"activation must be None or 'gelu', got {activation!r}")
     if len({t.device for t in (x, weight, offsets, bias) if t is not None}) > 1:
         raise ValueError("x, weight, offsets and bias must be on one device")
-    if x.is_cuda:
-        _check_gpu_product(x, weight)
-        if bias is not None and bias.dtype not in (torch.bfloat16, torch.float32):
-            raise ValueError(f"bias must be bf16 or fp32, got {bias.dtype}")
-    elif x.dtype != weight.dtype:
+    if x.dtype != weight.dtype:
         raise ValueError(f"x and weight must have one type, got {x.dtype} and {weight.dtype}")
 
 
@@ -130,35 +125,6 @@ def _ready(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-class _GroupedLinearHip(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, offsets, gelu):
-        x, weight = _ready(x), _ready(weight)
-        bias_in = None if bias is None else _ready(bias)
-        der = None
-        if gelu:
-            der = torch.empty(x.shape[0], weight.shape[1], dtype=x.dtype, device=x.device)
-        y = _C.ragged_nt(x, weight, offsets, bias_in, der, _GELU_DER if gelu else _PLAIN)
-        ctx.save_for_backward(x, weight, offsets, der)
-        ctx.bias_dtype = None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, offsets, der = ctx.saved_tensors
-        dp = _ready(dy) if der is None else _ready(dy) * der
-        dx = dw = db = None
-        if ctx.needs_input_grad[0]:
-            dx = _C.ragged_nn(dp, weight, offsets)
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dw = torch.empty_like(weight)
-            if ctx.needs_input_grad[2]:
-                db = torch.empty(weight.shape[:2], dtype=ctx.bias_dtype, device=weight.device)
-            _C.ragged_tn(dp, x, offsets, dw, db)
-        return dx, dw if ctx.needs_input_grad[1] else None, db, None, None
-
-
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
                    bias: Optional[torch.Tensor] = None,
                    activation: Optional[str] = None) -> torch.Tensor:
@@ -170,16 +136,10 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     Differentiable in x, weight and bias; a group without rows has zero weight
     gradients. Sums are fp32; y, dx and dW are rounded once (with gelu the
     gradient at its input is rounded to bf16 between the products)."""
+    if x.is_cuda and HAS_HIP:  # checks, gradients and all: bindings.cpp
+        return _C.grouped_linear(x, weight, offsets, bias, activation)
     _check_product(x, weight, offsets, bias, activation)
-    gelu = activation == "gelu"
-    if not (x.is_cuda and HAS_HIP):
-        return _grouped_linear_torch(x, weight, offsets, bias, gelu)
-    offsets = offsets.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (bias is not None and bias.requires_grad)):
-        return _GroupedLinearHip.apply(x, weight, bias, offsets, gelu)
-    return _C.ragged_nt(_ready(x), _ready(weight), offsets, None if bias is None else _ready(bias),
-                        None, _GELU if gelu else _PLAIN)
+    return _grouped_linear_torch(x, weight, offsets, bias, activation == "gelu")
 
 
 def _grouped_linear_torch(x, weight, offsets, bias, gelu):
@@ -203,7 +163,7 @@ class _RaggedFFNHip(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, offsets, stack):
-        der = torch.empty(x.shape[0], stack.ffn_dim, dtype=x.dtype, device=x.device)
+        der = torch.empty(x.shape[0], stack.ffn_dim, dtype=torch.float16, device=x.device)
         h = _C.ragged_nt(x, stack.W1c, offsets, stack.b1_f32, der, _GELU_DER)
         y = _C.ragged_nt(h, stack.W2c, offsets, stack.b2_f32, None, _PLAIN)
         ctx.save_for_backward(x, offsets, der, h)

@@ -70,6 +70,26 @@ def test_unaligned_and_strided():
         assert torch.equal(a, v * scale)
 
 
+def test_types_that_are_not_the_kernels():
+    """fp64 gradients, fp32 parameters, one of several not contiguous."""
+    ts = [torch.randn(100, device=DEV, dtype=torch.float64), torch.randn(7, device=DEV)]
+    want = norm64(ts)
+    norm, scale = Fops.grad_clip_scale(ts, 0.5)
+    assert (norm.double() - want).abs() <= NORM_TOL * want
+    mine = [t.clone() for t in ts]
+    Fops.clip_grad_norm_(mine, 0.5)
+    for a, t in zip(mine, ts):
+        assert torch.equal(a, t * scale)
+    m = [torch.randn(4, 6, device=DEV), torch.randn(5, device=DEV), torch.randn(6, 4, device=DEV).t()]
+    g = [torch.randn(4, 6, device=DEV), torch.randn(5, device=DEV).bfloat16(), torch.randn(4, 6, device=DEV)]
+    p = [m[0].clone(), m[1].bfloat16(), m[2].bfloat16()]
+    assert not p[2].is_contiguous()
+    want = [a - 0.1 * scale * b.float() for a, b in zip(m, g)]
+    Fops.master_sgd_step_(p, m, g, lr=0.1, grad_scale=scale)
+    for a, b, c in zip(m, want, p):
+        assert torch.allclose(a, b, rtol=2.0 ** -22, atol=1e-9) and torch.equal(c, a.to(c.dtype))
+
+
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 def test_not_finite(bad):
     ts = tensors([1000, 20000], [torch.float32])
@@ -213,10 +233,11 @@ def test_scale_on_a_side_stream():
 
 
 def test_refusals():
-    with pytest.raises(RuntimeError, match="bf16"):
-        from learning_at_home_amd.ops import _C
-
-        _C.grad_norm([torch.zeros(3, device=DEV, dtype=torch.float64)], 1.0, 1e-6)
+    with pytest.raises(ValueError, match="one device"):
+        Fops.grad_clip_scale([torch.zeros(3, device=DEV), torch.zeros(3)], 1.0)
+    with pytest.raises(ValueError, match="same shapes"):
+        Fops.master_sgd_step_([torch.zeros(3, device=DEV).bfloat16()], [torch.zeros(3, device=DEV)],
+                              [torch.zeros(4, device=DEV)], lr=0.1)
     torch.manual_seed(0)
     stack = ExpertStack(2, 256, 256).to(DEV)
     stack.init_gpu_state(master_weights=False)

@@ -52,8 +52,9 @@ def exact(x, w, b, offsets, dy, gelu):
         out["y"][s] = y.detach()
         tol["y"][s] = BF * y.detach().abs() + (1.13 * off + 2.0 ** -20 * u.detach().abs() if gelu else off)
         dp, = torch.autograd.grad(y, u, dy[s])
-        # with gelu: slope (its second derivative is at most 1) and dP are rounded to bf16 once each
-        doff = (2 * BF + BF * BF) * dp.abs() + dy[s].abs() * (off + 2.0 ** -20 + BF * 2.0 ** -8) * 1.01 if gelu else torch.zeros_like(dp)
+        # with gelu: the slope (its second derivative is at most 1) is rounded to fp16 (2^-11 of it, or
+        # 2^-25 where it is below fp16's normal range), dP to bf16
+        doff = (BF + 2.0 ** -11) * 1.01 * dp.abs() + dy[s].abs() * (off + 2.0 ** -20) * 1.01 if gelu else torch.zeros_like(dp)
         dx = dp @ w[e]
         out["dx"][s] = dx
         tol["dx"][s] = BF * dx.abs() + (doff @ w[e].abs()) * 1.01 + N * 2.0 ** -23 * (dp.abs() @ w[e].abs())
@@ -220,6 +221,56 @@ class TestGroupedLinear:
             y = Fops.grouped_linear(leaves[0], leaves[1], offsets, leaves[2])
             grad, = torch.autograd.grad(y, leaves[i], dy)
             assert torch.equal(grad, full[name])
+
+    @pytest.mark.parametrize("change,match", [
+        (dict(x=torch.zeros(4, 7).bfloat16()), "x must be"),
+        (dict(x=torch.zeros(4, 8)), "bf16"),
+        (dict(weight=torch.zeros(2, 9, 8).bfloat16()), "multiples of 8"),
+        (dict(weight=torch.zeros(2, 0, 8).bfloat16()), "empty"),
+        (dict(offsets=torch.tensor([0, 1, 4])), "offsets"),
+        (dict(offsets=torch.tensor([0, 4]).int()), "offsets"),
+        (dict(bias=torch.zeros(2, 8)), "bias"),
+        (dict(bias=torch.zeros(2, 16).half()), "bias"),
+        (dict(activation="relu"), "activation"),
+    ])
+    def test_refusals(self, change, match):
+        args = dict(x=torch.zeros(4, 8).bfloat16(), weight=torch.zeros(2, 16, 8).bfloat16(),
+                    offsets=torch.tensor([0, 1, 4]).int(), bias=None, activation=None)
+        args.update(change)
+        with pytest.raises(ValueError, match=match):
+            Fops.grouped_linear(*(t.to(DEV) if isinstance(t, torch.Tensor) else t for t in args.values()))
+
+    def test_refuses_two_devices_and_second_derivatives(self):
+        x, w, b, offsets, dy = problem([3, 2], 8, 16)
+        with pytest.raises(ValueError, match="one device"):
+            Fops.grouped_linear(x, w.cpu(), offsets)
+        x.requires_grad_(True)
+        y = Fops.grouped_linear(x, w, offsets)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(y, x, dy, create_graph=True)
+
+    @pytest.mark.parametrize("counts", [[5000, 1, 0, 3000], [0, 0, 70000], [300] * 16])
+    @pytest.mark.parametrize("gelu", [False, True])
+    def test_rows_in_parts(self, counts, gelu):
+        """Fewer tiles than CUs: each expert's rows are summed in parts and joined."""
+        p = problem(counts, 136, 72, tail=7, bias=torch.bfloat16)
+        want, tol = exact(*p, gelu)
+        got = run_all(*p, gelu)
+        for name in got:
+            close(name, got[name], want[name], tol[name])
+        again = run_all(*p, gelu)
+        for name in got:
+            assert torch.equal(got[name], again[name])
+
+    @pytest.mark.parametrize("counts", [[1], [0, 3, 0, 0, 1, 0], [2] * 20, [0] * 300 + [40], [1] * 4096])
+    @pytest.mark.parametrize("K,N", [(8, 8), (1000, 40), (256, 264)])
+    def test_few_rows(self, counts, K, N):
+        p = problem(counts, K, N, tail=2)
+        for gelu in (False, True):
+            want, tol = exact(*p, gelu)
+            with torch.no_grad():
+                y = Fops.grouped_linear(p[0], p[1], p[3], p[2], "gelu" if gelu else None)
+            close("y", y, want["y"], tol["y"])
 
     def test_same_bits_again(self):
         p = problem([300, 0, 77, 512], 256, 520, seed=3)
