@@ -73,6 +73,11 @@ LAH_DEVINL void wait_and_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+template <int N>
+LAH_DEVINL void wait_loads_and_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
 LAH_DEVINL void wait_reads_and_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 LAH_DEVINL void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
@@ -981,11 +986,6 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     if constexpr (X < 8) p0[X] = read_p(0, X);
     else q0[X - 8] = read_q(0, X - 8);
   };
-  auto read1 = [&](auto x) {
-    constexpr int X = decltype(x)::value;
-    if constexpr (X < 8) p1[X] = read_p(1, X);
-    else q1[X - 8] = read_q(1, X - 8);
-  };
 
   if (tiles >= 8 * stride)  // XCDs an eighth of a tile apart, so that their stores do not come all at once
     for (int i = (blockIdx.x & 7) * w.steps; i > 0; --i) __builtin_amdgcn_s_sleep(5);
@@ -1009,34 +1009,36 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     const bool with_db = KIND == R_TN && a.db != nullptr && w.n0 == 0;
     clear();
     for (int t = 0; t < w.steps; ++t) {
+      // Each quarter reads 8 fragments, early, for the next but one: at 128 bytes a cycle
+      // these and what comes in take three quarters of it.
       quarter(p0, q0, first_rows, true, with_db, [&](auto x) {
-        constexpr int X = decltype(x)::value;  // the last of them early enough to be there at the barrier
-        if constexpr (X < 4) {
-          read1(std::integral_constant<int, 2 * X>());
-          read1(std::integral_constant<int, 2 * X + 1>());
-        } else if constexpr (X < 12) {
-          read1(std::integral_constant<int, X + 4>());
-        }
+        constexpr int X = decltype(x)::value;
+        if constexpr (X < 8) p1[X] = read_p(1, X);
       });
-      wait_reads_and_barrier();  // nobody reads this stage any more
+      wait_reads_and_barrier();  // nobody reads this stage's P any more
       // A CU takes 64 bytes a cycle: a stage's loads keep it busy for half a stage, and
       // where they come faster the wave stands at the next one and multiplies nothing.
       quarter(p0, q0, last_rows, both, with_db, [&](auto x) {
         constexpr int X = decltype(x)::value;
+        if constexpr (X < 8) q1[X] = read_q(1, X);
         if constexpr (X % 3 == 0 && X < 15) load(std::integral_constant<int, X / 3>());
       });
       other_place();
+      // nor its Q, and P of the next stage has landed
+      if (stored) wait_and_barrier<(13 + STORES < 63 ? 13 + STORES : 63)>();
+      else wait_and_barrier<13>();
       quarter(p1, q1, first_rows, true, with_db, [&](auto x) {
         constexpr int X = decltype(x)::value;
+        if constexpr (X < 8) p0[X] = read_p(0, X);
         if constexpr (X % 3 == 0) load(std::integral_constant<int, 5 + X / 3>());
       });
-      // the next stage has landed
-      if (stored) wait_and_barrier<11 + STORES>();
-      else wait_and_barrier<11>();
+      // and its Q
+      if (stored) wait_loads_and_barrier<11 + STORES>();
+      else wait_loads_and_barrier<11>();
       stored = false;
       quarter(p1, q1, last_rows, both, with_db, [&](auto x) {
         constexpr int X = decltype(x)::value;
-        read0(x);
+        if constexpr (X < 8) q0[X] = read_q(0, X);
         if constexpr (X % 3 == 1 && X < 15) load(std::integral_constant<int, 11 + X / 3>());
         if constexpr (X == 15) next_stage();
       });
