@@ -594,15 +594,14 @@ LAH_DEVINL void pin_acc(f32x4& c) { asm volatile("" : "+a"(c)); }
 
 LAH_DEVINL void pin_vgpr(f32x4& c) { asm volatile("" : "+v"(c)); }
 
-// as lds_load16, to a place at a fixed distance
+// lds_load16 in two parts, to a place at a fixed distance: where, and one instruction
+// later (a matrix product, or s_nop) the load.
 template <int AT>
-LAH_DEVINL void lds_load16_at(i32x4 rsrc, unsigned voff, unsigned lds) {
-  asm volatile(
-      "s_add_u32 m0, %0, %3\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen lds"
-      ::"s"(lds), "v"(voff), "s"(rsrc), "n"(AT)
-      : "memory", "scc");
+LAH_DEVINL void lds_load_to(unsigned lds) {
+  asm volatile("s_add_u32 m0, %0, %1" ::"s"(lds), "n"(AT) : "memory", "scc");
+}
+LAH_DEVINL void lds_load_go(i32x4 rsrc, unsigned voff) {
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc) : "memory");
 }
 LAH_DEVINL bf16x8 lds_read16(unsigned at, int off) {
   return *(__attribute__((address_space(3))) const bf16x8*)(at + off);
@@ -618,8 +617,10 @@ template <typename F, int... X>
 LAH_DEVINL void each_of(F&& f, std::integer_sequence<int, X...>) {
   (f(std::integral_constant<int, X>()), ...);
 }
-template <typename F>
-LAH_DEVINL void each16(F&& f) { each_of(f, std::make_integer_sequence<int, 16>()); }
+template <int N, typename F>
+LAH_DEVINL void each(F&& f) { each_of(f, std::make_integer_sequence<int, N>()); }
+template <int N>
+using number = std::integral_constant<int, N>;
 
 struct BigTile {
   int e, part = 0, rows, steps, m0, n0;
@@ -645,14 +646,17 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   const int mine = stride % 256 == 0 ? (blockIdx.x & ~255) | ((blockIdx.x & 7) << 5) | ((blockIdx.x >> 3) & 31)
                                      : (int)blockIdx.x;
 
-  auto decode = [&](int L) {  // 8 M-tiles by all N-tiles at a time
+  // 4 M-tiles by all N-tiles at a time, so that an XCD has 4 by 8: 12 operand tiles for 32
+  // products, where 8 by 4 of experts of 4 M-tiles has 16 (256 experts of 1024 rows, 1024 ->
+  // 4096: 2022 us by 4, 2070 by 8, 2103 by 16; one expert 1891, 1967, 1957).
+  auto decode = [&](int L) {
     BigTile w;
     int q = L;
     if (KIND == R_TN) {
       w.e = L / (MT * NT);
       q = L % (MT * NT);
     }
-    const int first = q / (8 * NT) * 8, size = min(MT - first, 8), in = q % (8 * NT);
+    const int first = q / (4 * NT) * 4, size = min(MT - first, 4), in = q % (4 * NT);
     const int m = first + in % size;
     w.n0 = in / size * BN;
     if (KIND == R_TN) {
@@ -741,13 +745,20 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
       if (P_KC || Q_KC) mask_offsets();
     }
   };
-  auto load_p = [&](auto i) {
-    constexpr int I = decltype(i)::value;
-    lds_load16_at<I * BT * 16>(make_rsrc(pat, pbytes), pv[I], to);
+  // a stage's loads: 8 of P, 8 of Q
+  auto load_to = [&](auto x) {
+    constexpr int X = decltype(x)::value;
+    lds_load_to<(X < 8 ? 0 : BSLOT * 2) + (X & 7) * BT * 16>(to);
   };
-  auto load_q = [&](auto i) {
-    constexpr int I = decltype(i)::value;
-    lds_load16_at<BSLOT * 2 + I * BT * 16>(make_rsrc(qat, qbytes), qv[I], to);
+  auto load_go = [&](auto x) {
+    constexpr int X = decltype(x)::value;
+    if constexpr (X < 8) lds_load_go(make_rsrc(pat, pbytes), pv[X]);
+    else lds_load_go(make_rsrc(qat, qbytes), qv[X - 8]);
+  };
+  auto load = [&](auto x) {
+    load_to(x);
+    asm volatile("s_nop 0");
+    load_go(x);
   };
   // a tile's bias, with its first stage, by the first wave: loads are up to two tiles ahead
   auto stage_bias = [&](const BigTile& w, int turn) {
@@ -952,17 +963,22 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
 #pragma unroll
   for (int j = 0; j < 8; ++j) ones[j] = (__bf16)1.0f;
   asm volatile("" : "+v"(ones));  // not made anew before each product
-  // A quarter of a stage: 32 MFMAs, with `gap(x)`, x = 0 .. 15, behind every other. Those
-  // of the second rows (j0 = 4) are left out where a tile has none.
-  auto quarter = [&](const bf16x8(&p)[8], const bf16x8(&q)[8], auto j0_, bool there, bool with_db, auto gap) {
-    constexpr int j0 = decltype(j0_)::value;
+  // A quarter of a stage: 32 MFMAs. Behind the first 16, every other time, one of 8 LDS
+  // reads; `loads` loads from `load0` on, six MFMAs apart. More than three instructions
+  // behind one MFMA keep the next one waiting. The products of the second rows (j0 = 4)
+  // are left out where a tile has none.
+  auto quarter = [&](const bf16x8(&p)[8], const bf16x8(&q)[8], auto j0_, bool there, bool with_db, auto load0_,
+                     auto loads_, auto read) {
+    constexpr int j0 = decltype(j0_)::value, load0 = decltype(load0_)::value, loads = decltype(loads_)::value;
     if (j0 == 0 || there) {
-      each16([&](auto x) {
-        constexpr int X = decltype(x)::value, j = j0 + X / 4, i = X % 4 * 2;
-        mfma_acc(acc[i][j], p[i], q[j]);
-        mfma_acc(acc[i + 1][j], p[i + 1], q[j]);
+      each<32>([&](auto x) {
+        constexpr int X = decltype(x)::value, i = X % 8, j = j0 + X / 8, n = X / 6;
+        if constexpr (X % 6 == 1 && n < loads) load_to(number<load0 + n>());
         __builtin_amdgcn_sched_barrier(0);
-        gap(x);
+        mfma_acc(acc[i][j], p[i], q[j]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (X % 6 == 1 && n < loads) load_go(number<load0 + n>());
+        if constexpr (X < 16 && X % 2 == 0) read(number<X / 2>());
         __builtin_amdgcn_sched_barrier(0);
       });
       if (KIND == R_TN && with_db && wn == j0 / 4) {  // db: the sums of Q's columns
@@ -970,25 +986,14 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
         for (int j = 0; j < 4; ++j) mfma_vgpr(dbacc[j], ones, q[j0 + j]);
       }
     } else {
-      each16(gap);
+      each<8>(read);
+      each<loads>([&](auto x) { load(number<load0 + decltype(x)::value>()); });
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  const std::integral_constant<int, 0> first_rows;
-  const std::integral_constant<int, 4> last_rows;
-  auto load = [&](auto x) {
-    constexpr int X = decltype(x)::value;
-    if constexpr (X < 8) load_p(x);
-    else load_q(std::integral_constant<int, X - 8>());
-  };
-  auto read0 = [&](auto x) {
-    constexpr int X = decltype(x)::value;
-    if constexpr (X < 8) p0[X] = read_p(0, X);
-    else q0[X - 8] = read_q(0, X - 8);
-  };
+  const number<0> first_rows;
+  const number<4> last_rows;
 
-  if (tiles >= 8 * stride)  // XCDs an eighth of a tile apart, so that their stores do not come all at once
-    for (int i = (blockIdx.x & 7) * w.steps; i > 0; --i) __builtin_amdgcn_s_sleep(5);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     pv[i] = pv0[i];
@@ -996,11 +1001,12 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   }
   stage_bias(lw, 0);
   point_at(lw);
-  each16(load);
+  each<16>(load);
   next_stage();
-  each16(load);
+  each<16>(load);
   wait_and_barrier<16>();
-  each16(read0);
+  each<8>([&](auto x) { p0[decltype(x)::value] = read_p(0, decltype(x)::value); });
+  each<8>([&](auto x) { q0[decltype(x)::value] = read_q(0, decltype(x)::value); });
   next_stage();
   bool stored = false;  // the last tile's stores lie between this stage and the one before
   for (int at = mine, turn = 0; at < tiles; at += stride, ++turn) {
@@ -1011,37 +1017,26 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     for (int t = 0; t < w.steps; ++t) {
       // Each quarter reads 8 fragments, early, for the next but one: at 128 bytes a cycle
       // these and what comes in take three quarters of it.
-      quarter(p0, q0, first_rows, true, with_db, [&](auto x) {
-        constexpr int X = decltype(x)::value;
-        if constexpr (X < 8) p1[X] = read_p(1, X);
-      });
+      quarter(p0, q0, first_rows, true, with_db, number<0>(), number<0>(),
+              [&](auto x) { p1[decltype(x)::value] = read_p(1, decltype(x)::value); });
       wait_reads_and_barrier();  // nobody reads this stage's P any more
       // A CU takes 64 bytes a cycle: a stage's loads keep it busy for half a stage, and
       // where they come faster the wave stands at the next one and multiplies nothing.
-      quarter(p0, q0, last_rows, both, with_db, [&](auto x) {
-        constexpr int X = decltype(x)::value;
-        if constexpr (X < 8) q1[X] = read_q(1, X);
-        if constexpr (X % 3 == 0 && X < 15) load(std::integral_constant<int, X / 3>());
-      });
+      quarter(p0, q0, last_rows, both, with_db, number<0>(), number<5>(),
+              [&](auto x) { q1[decltype(x)::value] = read_q(1, decltype(x)::value); });
       other_place();
       // nor its Q, and P of the next stage has landed
       if (stored) wait_and_barrier<(13 + STORES < 63 ? 13 + STORES : 63)>();
       else wait_and_barrier<13>();
-      quarter(p1, q1, first_rows, true, with_db, [&](auto x) {
-        constexpr int X = decltype(x)::value;
-        if constexpr (X < 8) p0[X] = read_p(0, X);
-        if constexpr (X % 3 == 0) load(std::integral_constant<int, 5 + X / 3>());
-      });
+      quarter(p1, q1, first_rows, true, with_db, number<5>(), number<6>(),
+              [&](auto x) { p0[decltype(x)::value] = read_p(0, decltype(x)::value); });
       // and its Q
       if (stored) wait_loads_and_barrier<11 + STORES>();
       else wait_loads_and_barrier<11>();
       stored = false;
-      quarter(p1, q1, last_rows, both, with_db, [&](auto x) {
-        constexpr int X = decltype(x)::value;
-        if constexpr (X < 8) q0[X] = read_q(0, X);
-        if constexpr (X % 3 == 1 && X < 15) load(std::integral_constant<int, 11 + X / 3>());
-        if constexpr (X == 15) next_stage();
-      });
+      quarter(p1, q1, last_rows, both, with_db, number<11>(), number<5>(),
+              [&](auto x) { q0[decltype(x)::value] = read_q(0, decltype(x)::value); });
+      next_stage();
     }
     finish(w, turn);
     stored = true;
