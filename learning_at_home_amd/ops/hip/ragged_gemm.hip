@@ -622,6 +622,8 @@ LAH_DEVINL void each(F&& f) { each_of(f, std::make_integer_sequence<int, N>()); 
 template <int N>
 using number = std::integral_constant<int, N>;
 
+#define OUT_ROW 272  // bytes
+
 struct BigTile {
   int e, part = 0, rows, steps, m0, n0;
   long row0;
@@ -631,7 +633,8 @@ template <int KIND, int EPI>
 __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const int4* __restrict__ table) {
   constexpr bool P_KC = KIND == R_NT, Q_KC = KIND != R_TN;
   __shared__ __attribute__((aligned(16))) __bf16 smem[4 * BSLOT];
-  __shared__ __attribute__((aligned(16))) float bias_lds[4][BN];
+  __shared__ __attribute__((aligned(16))) float bias_lds[P_KC ? 4 : 1][BN];
+  __shared__ __attribute__((aligned(16))) char turn_lds[P_KC ? 1 : 4][16 * OUT_ROW];  // a wave's 16 rows of 256 bytes
 
   const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -691,7 +694,10 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   const int qc = Q_KC ? ((tid & 7) ^ kc_swz<2>(qr)) * 8 : ((tid & 15) ^ ks_swz(qr)) * 8;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    pv0[i] = P_KC ? (unsigned)((pr + i * 32) * a.K + pc) * 2
+    // KC: row 128 w + 8 l + f of P, fragment f's lane l, is row 128 w + 32 (f / 2) + 8 (l / 4) +
+    // 4 (f % 2) + l % 4 in LDS, where the reads have no conflicts
+    const int lr = pr + i * 32, pf = (lr >> 5 & 3) * 2 + (lr >> 2 & 1), pl = (lr >> 3 & 3) * 4 + (lr & 3);
+    pv0[i] = P_KC ? (unsigned)(((lr & 128) + pl * 8 + pf) * a.K + pc) * 2
                  : (unsigned)((pr + i * 8) * a.N + ((tid & 31) ^ ks_swz(pr + i * 8)) * 8) * 2;
     // KS: two tiles [64][128] beside each other
     qv0[i] = Q_KC ? (unsigned)((qr + i * 32) * a.K + qc) * 2
@@ -787,8 +793,8 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     settle();
   };
 
-  // P's fragment i, lane l15 of KC: row 128 wn + 32 (i / 2) + 8 (l15 / 4) + 4 (i % 2) + l15 % 4,
-  // so that a lane's results of fragments 2i, 2i + 1 are 8 neighbours, and 32 with the lanes g.
+  // P's fragment i, lane l15 of KC: row 128 wn + 8 l15 + i, so that a lane has 8 neighbouring
+  // outputs of a row and 16 lanes the wave's 128. KS: column 128 wn + 16 i + l15.
   // Q's fragment j: rows 32 j + 16 wm + l15, so that both halves of the waves have work in a
   // tile of few rows. The lanes' addresses are kept, and move between the two places by one
   // addition a stage: KC has one for each contraction half, KS one for each column base.
@@ -832,9 +838,11 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     hop = -hop;
   };
 
-  // ---- epilogue: lane (l15, g) holds rows 32 j + 16 wm + l15 of Q. Every lane stores
-  // every time, to a place past the descriptor's end where it has nothing: the wait
-  // counts on STORES of them.
+  // ---- epilogue: 256 bytes of 4 rows in a store. (64 bytes of 16 are written at 3.6 TB/s
+  // where these take 4.3: dW of 1024 experts of 32 rows, 2048 x 512, 590 us and 500.) KC has
+  // its results so: rows 4g .. 4g + 3 of Q's fragment, 8 columns. KS, with row l15 and columns
+  // 4g .. 4g + 3 of each fragment, turns them in LDS. Every lane stores every time, to a place
+  // past the descriptor's end where it has nothing: the wait counts on STORES of them.
   constexpr bool F32 = KIND == R_TN && EPI != R_BF16;
   constexpr int STORES = F32 || (KIND == R_NT && EPI == R_GELU_DER) ? 52 : 32;  // of 64: the counter goes to 63
   auto finish = [&](const BigTile& w, int turn) {
@@ -845,76 +853,89 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     const auto rc = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + base * (F32 ? 4 : 2), (short)0, 0x7fffffff, 0x00027000);
     const auto rd = __builtin_amdgcn_make_buffer_rsrc((char*)a.der + base * 2, (short)0, 0x7fffffff, 0x00027000);
     const int ncols = a.N - w.n0, nrows = KIND == R_TN ? a.M - w.m0 : w.rows;
-    float bias[KIND == R_NT ? 32 : 1];
-    if (KIND == R_NT) {
+    float bias[P_KC ? 8 : 1];
+    if (P_KC) {
 #pragma unroll
-      for (int x = 0; x < 32; ++x) {
-        const int n = wn * 128 + x / 8 * 32 + g * 8 + x % 8;
+      for (int x = 0; x < 8; ++x) {
+        const int n = wn * 128 + l15 * 8 + x;
         bias[x] = a.bias == nullptr ? 0.f
                   : a.bias_bf16     ? bf2f(((const __bf16*)bias_lds[turn & 3])[n])
                                     : bias_lds[turn & 3][n];
       }
     }
+    char* const turn_row = turn_lds[P_KC ? 0 : wave] + l15 * OUT_ROW;  // written by rows, 4 columns a lane
+    const char* const turn_at = turn_lds[P_KC ? 0 : wave] + g * OUT_ROW + l15 * 16;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) pin_acc(acc[i][j]);
-      const int r = j * 32 + wm * 16 + l15;
-      if (F32) {
+      const int r0 = j * 32 + wm * 16;
+      if (P_KC) {
+        const int n = wn * 128 + l15 * 8;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int n = wn * 128 + i * 16 + g * 4;
-          const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 4 : OOB_OFFSET;
-          f32x4 v = acc[i][j];
-          if (EPI == R_F32_ACC) v += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, off, 0, 0));
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rc, off, 0, 0);
-        }
-      } else {
-#pragma unroll
-        for (int ip = 0; ip < 4; ++ip) {
-          float v[8];
-#pragma unroll
-          for (int x = 0; x < 8; ++x) v[x] = acc[2 * ip + x / 4][j][x & 3];
-          int n;
-          if (P_KC) {
-            n = wn * 128 + ip * 32 + g * 8;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] += bias[ip * 8 + x];
-          } else {
-            // fragment 2 ip's columns 4g.. and 2 ip + 1's: lanes of odd g give the first and get the
-            // second, so that each has 8 neighbours
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[x]), __float_as_uint(v[4 + x]),
-                                                              false, false);
-              v[x] = __uint_as_float(s[0]);
-              v[4 + x] = __uint_as_float(s[1]);
-            }
-            n = wn * 128 + (2 * ip + (g & 1)) * 16 + (g >> 1) * 8;
-          }
+        for (int x = 0; x < 4; ++x) {
+          const int r = r0 + 4 * g + x;
           const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
           bf16x8 o;
           f16x8 d;
-          if (KIND == R_NN && EPI == R_MUL)
-            d = __builtin_bit_cast(f16x8, __builtin_amdgcn_raw_buffer_load_b128(rd, off, 0, 0));
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            if (KIND == R_NT && EPI == R_GELU) {
-              o[x] = f2bf(gelu_of(v[x]));
-            } else if (KIND == R_NT && EPI == R_GELU_DER) {
+          for (int i = 0; i < 8; ++i) {
+            const float v = acc[i][j][x] + bias[i];
+            if (EPI == R_GELU) {
+              o[i] = f2bf(gelu_of(v));
+            } else if (EPI == R_GELU_DER) {
               float y, s;
-              gelu_and_slope(v[x], &y, &s);
-              o[x] = f2bf(y);
-              d[x] = (_Float16)s;
-            } else if (KIND == R_NN && EPI == R_MUL) {
-              o[x] = f2bf(v[x] * (float)d[x]);
+              gelu_and_slope(v, &y, &s);
+              o[i] = f2bf(y);
+              d[i] = (_Float16)s;
             } else {
-              o[x] = f2bf(v[x]);
+              o[i] = f2bf(v);
             }
           }
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rc, off, 0, 0);
-          if (KIND == R_NT && EPI == R_GELU_DER)
+          if (EPI == R_GELU_DER)
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, d), rd, off, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < (F32 ? 2 : 1); ++h) {  // 256 bytes: 64 numbers of 32 bits or 128 of 16
+          if (F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(f32x4*)(turn_row + (i * 16 + g * 4) * 4) = acc[4 * h + i][j];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              bf16x4 o;
+              if (EPI != R_MUL) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[x] = f2bf(acc[i][j][x]);
+              } else {
+                typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+                const int r = r0 + l15, n = wn * 128 + i * 16 + g * 4;
+                const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
+                const f16x4 d = __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(rd, off, 0, 0));
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[x] = f2bf(acc[i][j][x] * (float)d[x]);
+              }
+              *(bf16x4*)(turn_row + (i * 16 + g * 4) * 2) = o;
+            }
+          }
+          const int n = wn * 128 + h * 64 + l15 * (F32 ? 4 : 8);
+          f32x4 turned[4];
+          // LDS works in the order of a wave's instructions; the compiler, who sees one lane, is to keep it
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int k = 0; k < 4; ++k) turned[k] = *(const f32x4*)(turn_at + 4 * k * OUT_ROW);
+          asm volatile("" ::: "memory");
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = r0 + 4 * k + g;
+            const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * (F32 ? 4 : 2) : OOB_OFFSET;
+            f32x4 v = turned[k];
+            if (KIND == R_TN && EPI == R_F32_ACC)
+              v += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, off, 0, 0));
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rc, off, 0, 0);
+          }
         }
       }
     }
@@ -975,7 +996,8 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
         constexpr int X = decltype(x)::value, i = X % 8, j = j0 + X / 8, n = X / 6;
         if constexpr (X % 6 == 1 && n < loads) load_to(number<load0 + n>());
         __builtin_amdgcn_sched_barrier(0);
-        mfma_acc(acc[i][j], p[i], q[j]);
+        if constexpr (P_KC) mfma_acc(acc[i][j], q[j], p[i]);
+        else mfma_acc(acc[i][j], p[i], q[j]);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (X % 6 == 1 && n < loads) load_go(number<load0 + n>());
         if constexpr (X < 16 && X % 2 == 0) read(number<X / 2>());
