@@ -262,6 +262,72 @@ class TestGroupedLinear:
         for name in got:
             assert torch.equal(got[name], again[name])
 
+    # tiles of fewer rows than their half, of all, of one more; one expert alone; none at all
+    @pytest.mark.parametrize("counts", [[20000, 1, 129, 0, 128, 127, 257, 15000], [0, 0, 36000], [0, 0, 0],
+                                        [i * 37 % 500 for i in range(140)]])
+    @pytest.mark.parametrize("K,N", [(520, 520), (8, 2056), (64, 2048), (2056, 8), (200, 1992)])
+    def test_large_tiles(self, counts, K, N):
+        """Many rows an expert and many tiles: forward, or dx, or both by the large tiles."""
+        p = problem(counts, K, N, tail=40 if sum(counts) else 40000, bias=torch.bfloat16 if K == 520 else torch.float32)
+        gelu = N != 2048
+        want, tol = exact(*p, gelu)
+        got = run_all(*p, gelu)
+        for name in got:
+            close(name, got[name], want[name], tol[name])
+        again = run_all(*p, gelu)
+        for name in got:
+            assert torch.equal(got[name], again[name])
+        with torch.no_grad():  # without the slope
+            y = Fops.grouped_linear(p[0], p[1], p[3], None if K == 8 else p[2], "gelu" if gelu else None)
+        if K == 8:
+            want, tol = exact(p[0], p[1], None, p[3], p[4], gelu)
+        close("y", y, want["y"], tol["y"])
+
+    def test_large_tiles_keep_to_their_rows(self):
+        x, w, b, offsets, dy = problem([20000, 300, 0, 16000], 264, 520, tail=300)
+        end = 36300
+        clean = run_all(x, w, b, offsets, dy, True)
+        assert not clean["y"][end:].any() and not clean["dx"][end:].any()
+        x2, dy2, w2 = x.clone(), dy.clone(), w.clone()
+        x2[end:], dy2[end:] = float("nan"), float("inf")
+        w2[2] = float("nan")
+        got = run_all(x2, w2, b, offsets, dy2, True)
+        for name in got:
+            assert torch.equal(got[name], clean[name]), name
+
+    def test_large_tiles_captured_and_beside_others(self):
+        """Graphs of different sizes, replayed at once on two streams, with eager work between."""
+        cases = []
+        for counts, K, N in (([20000, 300, 0, 16000], 264, 520), ([3000, 5000], 128, 72), ([9000, 30000], 520, 600)):
+            x, w, b, offsets, dy = problem(counts, K, N, tail=300)
+            leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+            def step(x=x, w=w, b=b, offsets=offsets, dy=dy, leaves=leaves):
+                y = Fops.grouped_linear(x, w, offsets, b, "gelu")
+                return (y, *torch.autograd.grad(y, leaves, dy))
+
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                step()
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                held = step()
+            cases.append((graph, held, step, side, dy))
+        for i in range(3):
+            for _, _, _, _, dy in cases:
+                dy.add_(i)
+            torch.cuda.synchronize()
+            for graph, _, _, side, _ in cases:
+                with torch.cuda.stream(side):
+                    graph.replay()
+            now = [step() for _, _, step, _, _ in cases]
+            torch.cuda.synchronize()
+            for (_, held, _, _, _), eager in zip(cases, now):
+                for a, b_ in zip(held, eager):
+                    assert torch.equal(a, b_)
+
     @pytest.mark.parametrize("counts", [[1], [0, 3, 0, 0, 1, 0], [2] * 20, [0] * 300 + [40], [1] * 4096])
     @pytest.mark.parametrize("K,N", [(8, 8), (1000, 40), (256, 264)])
     def test_few_rows(self, counts, K, N):
@@ -351,9 +417,10 @@ def make_stack(E, d, ffn, seed=0):
 
 
 class TestRaggedFFN:
-    @pytest.mark.parametrize("counts", [[5, 0, 130, 64], [0, 1, 0, 0], [300, 300, 1, 2]])
+    @pytest.mark.parametrize("counts", [[5, 0, 130, 64], [0, 1, 0, 0], [300, 300, 1, 2], [3000, 0, 9000, 1],
+                                        [20000, 18000, 0, 300]])
     def test_against_double(self, counts):
-        stack = make_stack(4, 128, 256)
+        stack = make_stack(4, 128, 512 if sum(counts) > 30000 else 256)
         offsets = offsets_of(counts)
         R = sum(counts) + 3
         x = torch.randn(R, 128, device=DEV).bfloat16().requires_grad_(True)
