@@ -14,7 +14,10 @@
 // chain of small steps in each.
 #include "common.h"
 
-#define LY_ITER 4  // 64-slot groups a wave
+// 64-slot groups a wave: more blocks while there are few, shorter tables when there are many.
+// 98304 slots, 256 experts: 9.6 us by 2 and 12.1 by 4; 65536, 1024: 12.6 and 13.9; 400000, 256:
+// 14.9 and 14.4; 1500000, 256: 66 and 43. Up to 4096 one block has all by 4: 7.3 us, 9.2 by 2.
+static int layout_groups(long n) { return n > 4096 && n <= 262144 ? 2 : 4; }
 
 template <typename Id>
 LAH_DEVINL int id_of(const Id* ids, long s, long n, int E) {
@@ -61,20 +64,20 @@ __launch_bounds__(64) __global__ void layout_prefix_kernel(int* __restrict__ tab
 
 enum { LY_ONE = 0, LY_SUM = 1, LY_PREFIX = 2 };  // one block; sums the table itself; prefix kernel ran
 
-template <typename Id, int ECAP, int WAVES, int MODE>
+template <typename Id, int ECAP, int WAVES, int GROUPS, int MODE>
 __launch_bounds__(WAVES * 64) __global__
 void layout_place_kernel(const Id* __restrict__ ids, long n, int E, int bits, const int* __restrict__ table,
                          int* __restrict__ offsets, int* __restrict__ order, int* __restrict__ rows) {
-  constexpr int T = WAVES * 64, CH = T * LY_ITER, PER = ECAP / T > 0 ? ECAP / T : 1;
+  constexpr int T = WAVES * 64, CH = T * GROUPS, PER = ECAP / T > 0 ? ECAP / T : 1;
   __shared__ unsigned short wh[WAVES][ECAP];  // a wave's counts, then those of the waves before it
   __shared__ int start[ECAP], total[ECAP];
   __shared__ int wsum[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x, B = gridDim.x;
-  const long s0 = (long)b * CH + wave * (64 * LY_ITER) + lane;
+  const long s0 = (long)b * CH + wave * (64 * GROUPS) + lane;
 
-  int id[LY_ITER], rank[LY_ITER];
+  int id[GROUPS], rank[GROUPS];
 #pragma unroll
-  for (int i = 0; i < LY_ITER; ++i) id[i] = id_of(ids, s0 + i * 64, n, E);
+  for (int i = 0; i < GROUPS; ++i) id[i] = id_of(ids, s0 + i * 64, n, E);
   for (int e = lane; e < E; e += 64) wh[wave][e] = 0;
   for (int e = tid; e < E; e += T) start[e] = total[e] = 0;
   __syncthreads();
@@ -108,7 +111,7 @@ void layout_place_kernel(const Id* __restrict__ ids, long n, int E, int bits, co
   }
 
 #pragma unroll
-  for (int i = 0; i < LY_ITER; ++i) {
+  for (int i = 0; i < GROUPS; ++i) {
     const int e = id[i];
     unsigned long long peers = ~0ull;
     for (int q = 0; q < bits; ++q) {
@@ -170,7 +173,7 @@ void layout_place_kernel(const Id* __restrict__ ids, long n, int E, int bits, co
   __syncthreads();
 
 #pragma unroll
-  for (int i = 0; i < LY_ITER; ++i) {
+  for (int i = 0; i < GROUPS; ++i) {
     const long s = s0 + i * 64;
     if (s < n) {
       int r = -1;
@@ -184,41 +187,48 @@ void layout_place_kernel(const Id* __restrict__ ids, long n, int E, int bits, co
   for (long r = valid + (long)b * T + tid; r < n; r += (long)B * T) order[r] = -1;
 }
 
-template <typename Id, int ECAP, int WAVES>
+template <typename Id, int ECAP, int WAVES, int GROUPS>
 static void launch_layout(const Id* ids, long n, int E, int* table, int* offsets, int* order, int* rows,
                           hipStream_t stream) {
-  constexpr int CH = WAVES * 64 * LY_ITER;
+  constexpr int CH = WAVES * 64 * GROUPS;
   const int B = (int)((n + CH - 1) / CH);
   int bits = 0;
   while ((1 << bits) <= E) ++bits;
   dim3 grid(B < 1 ? 1 : B), block(WAVES * 64);
   if (B <= 1) {
-    hipLaunchKernelGGL((layout_place_kernel<Id, ECAP, WAVES, LY_ONE>), grid, block, 0, stream, ids, n, E,
+    hipLaunchKernelGGL((layout_place_kernel<Id, ECAP, WAVES, GROUPS, LY_ONE>), grid, block, 0, stream, ids, n, E,
                        bits, table, offsets, order, rows);
     return;
   }
   hipLaunchKernelGGL((layout_count_kernel<Id, CH>), grid, dim3(1024), 0, stream, ids, n, E, table);
   if ((long)B * E <= 65536) {
-    hipLaunchKernelGGL((layout_place_kernel<Id, ECAP, WAVES, LY_SUM>), grid, block, 0, stream, ids, n, E,
+    hipLaunchKernelGGL((layout_place_kernel<Id, ECAP, WAVES, GROUPS, LY_SUM>), grid, block, 0, stream, ids, n, E,
                        bits, table, offsets, order, rows);
   } else {
     hipLaunchKernelGGL(layout_prefix_kernel, dim3(cdiv(E, 64)), dim3(64), 0, stream, table, B, E);
-    hipLaunchKernelGGL((layout_place_kernel<Id, ECAP, WAVES, LY_PREFIX>), grid, block, 0, stream, ids, n,
+    hipLaunchKernelGGL((layout_place_kernel<Id, ECAP, WAVES, GROUPS, LY_PREFIX>), grid, block, 0, stream, ids, n,
                        E, bits, table, offsets, order, rows);
   }
+}
+
+template <typename Id, int ECAP, int WAVES>
+static void layout_sized(const Id* ids, long n, int E, int* table, int* offsets, int* order, int* rows,
+                         hipStream_t stream) {
+  if (layout_groups(n) == 2) launch_layout<Id, ECAP, WAVES, 2>(ids, n, E, table, offsets, order, rows, stream);
+  else launch_layout<Id, ECAP, WAVES, 4>(ids, n, E, table, offsets, order, rows, stream);
 }
 
 template <typename Id>
 static void layout_any(const Id* ids, long n, int E, int* table, int* offsets, int* order, int* rows,
                        hipStream_t stream) {
-  if (E <= 256) launch_layout<Id, 256, 16>(ids, n, E, table, offsets, order, rows, stream);
-  else if (E <= 1024) launch_layout<Id, 1024, 16>(ids, n, E, table, offsets, order, rows, stream);
-  else launch_layout<Id, 4096, 8>(ids, n, E, table, offsets, order, rows, stream);
+  if (E <= 256) layout_sized<Id, 256, 16>(ids, n, E, table, offsets, order, rows, stream);
+  else if (E <= 1024) layout_sized<Id, 1024, 16>(ids, n, E, table, offsets, order, rows, stream);
+  else layout_sized<Id, 4096, 8>(ids, n, E, table, offsets, order, rows, stream);
 }
 
 // whole numbers the table needs: a row a block, and one of sums
 extern "C" long lah_ragged_layout_table(long n, int E) {
-  const long ch = (E <= 1024 ? 16 : 8) * 64 * LY_ITER, B = (n + ch - 1) / ch;
+  const long ch = (E <= 1024 ? 16 : 8) * 64 * layout_groups(n), B = (n + ch - 1) / ch;
   return B <= 1 ? 0 : (B + 1) * E;
 }
 
