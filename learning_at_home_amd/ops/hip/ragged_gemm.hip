@@ -53,6 +53,14 @@ LAH_DEVINL i32x4 make_rsrc(const void* p, int bytes) {
   r[3] = 0x00027000;
   return r;
 }
+// A load in asm may not read a scalar register that a vector instruction (such as the
+// readfirstlane above) wrote less than five instructions ago, and the compiler does not look
+// into it: the descriptor is held in scalar registers from here on, and five stand between.
+LAH_DEVINL i32x4 settled_rsrc(const void* p, int bytes) {
+  i32x4 r = make_rsrc(p, bytes);
+  asm volatile("s_nop 4" : "+s"(r));
+  return r;
+}
 #define OOB_OFFSET 0x80000000u  // past every descriptor made here
 
 // Global -> LDS without registers, 16 bytes a lane, to lds + lane * 16. In asm,
@@ -233,20 +241,20 @@ __launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
     const unsigned to = lds0 + (p % 3) * (SLOT * 2);
     if (P_KC) {
       const int skip = h * 16 * a.K + t * 64;
-      const i32x4 r = make_rsrc(Pb + skip, max(pbytes - skip * 2, 0));  // few columns: no second half
+      const i32x4 r = settled_rsrc(Pb + skip, max(pbytes - skip * 2, 0));  // few columns: no second half
       const int left = a.K - t * 64;
 #pragma unroll
       for (int i = 0; i < 4; ++i) lds_load16(r, pcc[i] >= left ? OOB_OFFSET : pv[i], to + i * RT * 16);
     } else {
       const int left = max(min(a.K - p * RBK, RBK), 0);
-      const i32x4 r = make_rsrc(Pb + (long)p * RBK * a.N, left > 0 ? (left * a.N - n0) * 2 : 0);
+      const i32x4 r = settled_rsrc(Pb + (long)p * RBK * a.N, left > 0 ? (left * a.N - n0) * 2 : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) lds_load16(r, pv[i], to + i * RT * 16);
     }
   };
   auto stage_q = [&](int t) {
     const unsigned to = lds0 + (3 + (t & 1)) * (SLOT * 2);
-    const i32x4 r = make_rsrc(Qb + t * 64, qbytes - t * 128);
+    const i32x4 r = settled_rsrc(Qb + t * 64, qbytes - t * 128);
     const int left = a.K - t * 64;  // chunks past the contraction's end give zeros
 #pragma unroll
     for (int i = 0; i < 4; ++i) lds_load16(r, cc[i] >= left ? OOB_OFFSET : qv[i], to + i * RT * 16);
@@ -756,22 +764,26 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     constexpr int X = decltype(x)::value;
     lds_load_to<(X < 8 ? 0 : BSLOT * 2) + (X & 7) * BT * 16>(to);
   };
-  auto load_go = [&](auto x) {
+  auto load_go = [&](auto x, i32x4 p, i32x4 q) {
     constexpr int X = decltype(x)::value;
-    if constexpr (X < 8) lds_load_go(make_rsrc(pat, pbytes), pv[X]);
-    else lds_load_go(make_rsrc(qat, qbytes), qv[X - 8]);
+    if constexpr (X < 8) lds_load_go(p, pv[X]);
+    else lds_load_go(q, qv[X - 8]);
   };
-  auto load = [&](auto x) {
+  auto load = [&](auto x, i32x4 p, i32x4 q) {
     load_to(x);
     asm volatile("s_nop 0");
-    load_go(x);
+    load_go(x, p, q);
+  };
+  auto load_all = [&]() {
+    const i32x4 p = settled_rsrc(pat, pbytes), q = settled_rsrc(qat, qbytes);
+    each<16>([&](auto x) { load(x, p, q); });
   };
   // a tile's bias, with its first stage, by the first wave: loads are up to two tiles ahead
   auto stage_bias = [&](const BigTile& w, int turn) {
     if (KIND == R_NT && a.bias != nullptr && wave == 0) {
       const int size = a.bias_bf16 ? 2 : 4;
       const char* at = (const char*)a.bias + ((long)w.e * a.N + w.n0) * size;
-      const i32x4 r = make_rsrc(at, w.e == a.E ? 0 : min(a.N - w.n0, BN) * size);
+      const i32x4 r = settled_rsrc(at, w.e == a.E ? 0 : min(a.N - w.n0, BN) * size);
       lds_load16(r, lane * 16, bias0 + (turn & 3) * (BN * 4));
     }
   };
@@ -985,21 +997,34 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   for (int j = 0; j < 8; ++j) ones[j] = (__bf16)1.0f;
   asm volatile("" : "+v"(ones));  // not made anew before each product
   // A quarter of a stage: 32 MFMAs. Behind the first 16, every other time, one of 8 LDS
-  // reads; `loads` loads from `load0` on, six MFMAs apart. More than three instructions
-  // behind one MFMA keep the next one waiting. The products of the second rows (j0 = 4)
-  // are left out where a tile has none.
+  // reads; `loads` loads from `load0` on, five MFMAs apart, the first behind the fourth: five
+  // instructions and more behind its descriptor (settled_rsrc). More than three instructions
+  // behind one MFMA keep the next one waiting. The products of the second rows (j0 = 4) are
+  // left out where a tile has none. (Left out by 64 rows instead of 128 they cost more
+  // branches than they save: 256 experts of 1024 rows in the mean, 1024 -> 4096, 2068 us and
+  // 2043.)
   auto quarter = [&](const bf16x8(&p)[8], const bf16x8(&q)[8], auto j0_, bool there, bool with_db, auto load0_,
                      auto loads_, auto read) {
     constexpr int j0 = decltype(j0_)::value, load0 = decltype(load0_)::value, loads = decltype(loads_)::value;
+    i32x4 rp{}, rq{};
+    if constexpr (load0 < 8 && loads > 0) {
+      rp = make_rsrc(pat, pbytes);
+      asm volatile("" : "+s"(rp));
+    }
+    if constexpr (load0 + loads > 8) {
+      rq = make_rsrc(qat, qbytes);
+      asm volatile("" : "+s"(rq));
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if (j0 == 0 || there) {
       each<32>([&](auto x) {
-        constexpr int X = decltype(x)::value, i = X % 8, j = j0 + X / 8, n = X / 6;
-        if constexpr (X % 6 == 1 && n < loads) load_to(number<load0 + n>());
+        constexpr int X = decltype(x)::value, i = X % 8, j = j0 + X / 8, n = X / 5;
+        if constexpr (X % 5 == 3 && n < loads) load_to(number<load0 + n>());
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (P_KC) mfma_acc(acc[i][j], q[j], p[i]);
         else mfma_acc(acc[i][j], p[i], q[j]);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (X % 6 == 1 && n < loads) load_go(number<load0 + n>());
+        if constexpr (X % 5 == 3 && n < loads) load_go(number<load0 + n>(), rp, rq);
         if constexpr (X < 16 && X % 2 == 0) read(number<X / 2>());
         __builtin_amdgcn_sched_barrier(0);
       });
@@ -1008,8 +1033,9 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
         for (int j = 0; j < 4; ++j) mfma_vgpr(dbacc[j], ones, q[j0 + j]);
       }
     } else {
-      each<8>(read);
-      each<loads>([&](auto x) { load(number<load0 + decltype(x)::value>()); });
+      each<8>(read);  // these stand between the descriptor and the loads
+      __builtin_amdgcn_sched_barrier(0);
+      each<loads>([&](auto x) { load(number<load0 + decltype(x)::value>(), rp, rq); });
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -1023,9 +1049,9 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   }
   stage_bias(lw, 0);
   point_at(lw);
-  each<16>(load);
+  load_all();
   next_stage();
-  each<16>(load);
+  load_all();
   wait_and_barrier<16>();
   each<8>([&](auto x) { p0[decltype(x)::value] = read_p(0, decltype(x)::value); });
   each<8>([&](auto x) { q0[decltype(x)::value] = read_q(0, decltype(x)::value); });
