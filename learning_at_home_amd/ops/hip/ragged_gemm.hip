@@ -789,12 +789,20 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   };
 
   f32x4 acc[8][8], dbacc[4];
-  auto clear = [&]() {
+  auto begin = [&](int turn) {  // at the bias of a lane's 8 columns
+    float bias[8] = {};
+    if (P_KC && a.bias != nullptr) {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const int n = wn * 128 + l15 * 8 + x;
+        bias[x] = a.bias_bf16 ? bf2f(((const __bf16*)bias_lds[turn & 3])[n]) : bias_lds[turn & 3][n];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+        acc[i][j] = {bias[i], bias[i], bias[i], bias[i]};
         pin_acc(acc[i][j]);
       }
 #pragma unroll
@@ -857,7 +865,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   // past the descriptor's end where it has nothing: the wait counts on STORES of them.
   constexpr bool F32 = KIND == R_TN && EPI != R_BF16;
   constexpr int STORES = F32 || (KIND == R_NT && EPI == R_GELU_DER) ? 52 : 32;  // of 64: the counter goes to 63
-  auto finish = [&](const BigTile& w, int turn) {
+  auto finish = [&](const BigTile& w) {
     int l15 = lane & 15, g = lane >> 4;
     asm volatile("" : "+v"(l15), "+v"(g));  // offsets made from these are not kept through the loop
     settle();
@@ -865,16 +873,6 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     const auto rc = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + base * (F32 ? 4 : 2), (short)0, 0x7fffffff, 0x00027000);
     const auto rd = __builtin_amdgcn_make_buffer_rsrc((char*)a.der + base * 2, (short)0, 0x7fffffff, 0x00027000);
     const int ncols = a.N - w.n0, nrows = KIND == R_TN ? a.M - w.m0 : w.rows;
-    float bias[P_KC ? 8 : 1];
-    if (P_KC) {
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const int n = wn * 128 + l15 * 8 + x;
-        bias[x] = a.bias == nullptr ? 0.f
-                  : a.bias_bf16     ? bf2f(((const __bf16*)bias_lds[turn & 3])[n])
-                                    : bias_lds[turn & 3][n];
-      }
-    }
     char* const turn_row = turn_lds[P_KC ? 0 : wave] + l15 * OUT_ROW;  // written by rows, 4 columns a lane
     const char* const turn_at = turn_lds[P_KC ? 0 : wave] + g * OUT_ROW + l15 * 16;
 #pragma unroll
@@ -892,7 +890,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
           f16x8 d;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float v = acc[i][j][x] + bias[i];
+            const float v = acc[i][j][x];
             if (EPI == R_GELU) {
               o[i] = f2bf(gelu_of(v));
             } else if (EPI == R_GELU_DER) {
@@ -1061,7 +1059,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     if (turn > 0) w = decode(at);
     const bool both = KIND == R_TN || w.rows > 128;  // the tile's second half of rows is there
     const bool with_db = KIND == R_TN && a.db != nullptr && w.n0 == 0;
-    clear();
+    begin(turn);
     for (int t = 0; t < w.steps; ++t) {
       // Each quarter reads 8 fragments, early, for the next but one: at 128 bytes a cycle
       // these and what comes in take three quarters of it.
@@ -1086,7 +1084,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
               [&](auto x) { q0[decltype(x)::value] = read_q(0, decltype(x)::value); });
       next_stage();
     }
-    finish(w, turn);
+    finish(w);
     stored = true;
   }
   // nothing may come into this block's LDS once it is another's
