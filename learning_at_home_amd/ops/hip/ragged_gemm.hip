@@ -75,6 +75,16 @@ LAH_DEVINL void lds_load16(i32x4 rsrc, unsigned voff, unsigned lds) {
       : "memory");
 }
 
+// the same, of what need not stay in L2
+LAH_DEVINL void lds_load16_once(i32x4 rsrc, unsigned voff, unsigned lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen nt lds"
+      ::"s"(lds), "v"(voff), "s"(rsrc)
+      : "memory");
+}
+
 // All LDS reads of this wave done and at most N loads in flight, then the barrier.
 template <int N>
 LAH_DEVINL void wait_and_barrier() {
@@ -160,6 +170,7 @@ struct RaggedArgs {
   int E, N, M, K;    // K: contraction of NT / NN
   int bias_bf16;     // of bias, or of db
   int splits;        // TN: parts of each expert's rows, each with sums of its own
+  bool once;         // weights that no cache holds until they are read again
 };
 
 // Blocks go to the 8 XCDs in turn: of each 512, the 64 that share one XCD (two a
@@ -236,6 +247,15 @@ __launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
   for (int i = 0; i < 4; ++i) pcc[i] = ((i * RT + tid) & 7 ^ kc_swz<4>((i * RT + tid) >> 3)) * 8;
   const unsigned lds0 = lds_addr(smem) + wave * 1024;
 
+  auto load4 = [&](const i32x4& r, auto at, unsigned to) {
+    if (a.once) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lds_load16_once(r, at(i), to + i * RT * 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lds_load16(r, at(i), to + i * RT * 16);
+    }
+  };
   auto stage_p = [&](int p) {  // phase p's part, to slot p % 3
     const int t = p >> 1, h = p & 1;
     const unsigned to = lds0 + (p % 3) * (SLOT * 2);
@@ -243,13 +263,11 @@ __launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
       const int skip = h * 16 * a.K + t * 64;
       const i32x4 r = settled_rsrc(Pb + skip, max(pbytes - skip * 2, 0));  // few columns: no second half
       const int left = a.K - t * 64;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lds_load16(r, pcc[i] >= left ? OOB_OFFSET : pv[i], to + i * RT * 16);
+      load4(r, [&](int i) { return pcc[i] >= left ? OOB_OFFSET : pv[i]; }, to);
     } else {
       const int left = max(min(a.K - p * RBK, RBK), 0);
       const i32x4 r = settled_rsrc(Pb + (long)p * RBK * a.N, left > 0 ? (left * a.N - n0) * 2 : 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lds_load16(r, pv[i], to + i * RT * 16);
+      load4(r, [&](int i) { return pv[i]; }, to);
     }
   };
   auto stage_q = [&](int t) {
@@ -1107,6 +1125,12 @@ static bool launch_few(const RaggedArgs& a, hipStream_t stream) {
   return true;
 }
 
+// Weights larger than the last cache (256 MB) are gone before the next call, and where
+// experts have few rows each is read once or twice: such loads leave L2 to the rows. 1024
+// experts of 32 rows, 2048 -> 512: 434 us, 467 without; 256 of 8, 1024 -> 4096: 334 and 360,
+// its dx 346 and 383. Smaller weights lose by it: 64 of 1024 x 1024, 64 rows each, 42 and 39.
+static bool read_once(int E, int N, int K) { return (long)E * N * K * 2 > (256l << 20); }
+
 template <int KIND, int EPI>
 static void launch_rows(const RaggedArgs& a, void* table, hipStream_t stream) {
   if constexpr (KIND == R_NT)
@@ -1163,7 +1187,7 @@ extern "C" void lah_ragged_nt(const void* x, const void* w, void* y, const void*
                               const void* bias, int bias_bf16, void* der, long R, int E, int N,
                               int K, int epi, void* table, hipStream_t stream) {
   RaggedArgs a{(const __bf16*)w, (const __bf16*)x, y, (const int*)offsets, bias, (_Float16*)der,
-               nullptr, R, E, N, 0, K, bias_bf16, 1};
+               nullptr, R, E, N, 0, K, bias_bf16, 1, read_once(E, N, K)};
   if (epi == R_GELU_DER) launch_rows<R_NT, R_GELU_DER>(a, table, stream);
   else if (epi == R_GELU) launch_rows<R_NT, R_GELU>(a, table, stream);
   else launch_rows<R_NT, R_PLAIN>(a, table, stream);
@@ -1174,7 +1198,7 @@ extern "C" void lah_ragged_nn(const void* d, const void* w, void* out, const voi
                               void* der, long R, int E, int N, int K, void* table,
                               hipStream_t stream) {
   RaggedArgs a{(const __bf16*)w, (const __bf16*)d, out, (const int*)offsets, nullptr,
-               (_Float16*)der, nullptr, R, E, N, 0, K, 0, 1};
+               (_Float16*)der, nullptr, R, E, N, 0, K, 0, 1, read_once(E, N, K)};
   if (der != nullptr) launch_rows<R_NN, R_MUL>(a, table, stream);
   else launch_rows<R_NN, R_PLAIN>(a, table, stream);
 }
@@ -1193,7 +1217,7 @@ extern "C" void lah_ragged_tn(const void* d, const void* x, void* dw, void* db, 
                               const void* offsets, long R, int E, int N, int M, int out, int splits,
                               void* part, hipStream_t stream) {
   RaggedArgs a{(const __bf16*)x, (const __bf16*)d, dw, (const int*)offsets, nullptr, nullptr,
-               db, R, E, N, M, 0, db_bf16, splits};
+               db, R, E, N, M, 0, db_bf16, splits, false};
   if (splits > 1) {
     const long n = (long)E * M * N;
     float* db_part = (float*)part + splits * n;

@@ -283,6 +283,14 @@ class TestGroupedLinear:
             want, tol = exact(p[0], p[1], None, p[3], p[4], gelu)
         close("y", y, want["y"], tol["y"])
 
+    def test_weights_past_the_cache(self):
+        p = problem([3] * 38 + [0, 140], 2056, 2048, tail=3)
+        assert p[1].numel() * 2 > 256 << 20
+        want, tol = exact(*p, True)
+        got = run_all(*p, True)
+        for name in got:
+            close(name, got[name], want[name], tol[name])
+
     def test_large_tiles_keep_to_their_rows(self):
         x, w, b, offsets, dy = problem([20000, 300, 0, 16000], 264, 520, tail=300)
         end = 36300
