@@ -49,6 +49,7 @@ void lah_ragged_nt(const void*, const void*, void*, const void*, const void*, in
 void lah_ragged_nn(const void*, const void*, void*, const void*, void*, long, int, int, int,
                    void*, hipStream_t);
 int lah_ragged_splits(long, int, int, int);
+long lah_ragged_order_room(long, int, int, int, int);
 void lah_ragged_tn(const void*, const void*, void*, void*, int, const void*, long, int, int,
                    int, int, int, void*, hipStream_t);
 void lah_ragged_slope(const void*, const void*, void*, long, hipStream_t);
@@ -532,10 +533,12 @@ void ragged_tn(torch::Tensor d, torch::Tensor x, torch::Tensor offsets, torch::T
   }
   ON_DEVICE_OF(d);
   const int splits = lah_ragged_splits(R, (int)E, (int)N, (int)M);
-  torch::Tensor part;
-  if (splits > 1) part = torch::empty({splits * E * M * (N + 1)}, d.options().dtype(at::kFloat));
+  const long order = lah_ragged_order_room(R, (int)E, (int)N, (int)M, splits);
+  torch::Tensor work;
+  if (splits > 1) work = torch::empty({splits * E * M * (N + 1)}, d.options().dtype(at::kFloat));
+  else if (order > 0) work = torch::empty({order}, d.options().dtype(at::kInt));
   lah_ragged_tn(d.data_ptr(), x.data_ptr(), dw.data_ptr(), db_p, db_bf16, offsets.data_ptr(), R,
-                (int)E, (int)N, (int)M, bf16 ? 2 : accumulate ? 1 : 0, splits, ptr_or_null(part),
+                (int)E, (int)N, (int)M, bf16 ? 2 : accumulate ? 1 : 0, splits, ptr_or_null(work),
                 cur_stream());
   CHECK_LAUNCH();
 }

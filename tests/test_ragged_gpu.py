@@ -283,6 +283,15 @@ class TestGroupedLinear:
             want, tol = exact(p[0], p[1], None, p[3], p[4], gelu)
         close("y", y, want["y"], tol["y"])
 
+    @pytest.mark.parametrize("counts", [[0, 3000, 1, 700, 700, 0, 20000, 64, 65] * 8, [300] * 65, [0] * 69 + [30000]])
+    def test_weight_gradients_by_rows(self, counts):
+        """More tiles than blocks, experts of very different rows."""
+        p = problem(counts, 264, 776, tail=9)
+        want, tol = exact(*p, False)
+        got = run_all(*p, False)
+        for name in got:
+            close(name, got[name], want[name], tol[name])
+
     def test_weights_past_the_cache(self):
         p = problem([3] * 38 + [0, 140], 2056, 2048, tail=3)
         assert p[1].numel() * 2 > 256 << 20
