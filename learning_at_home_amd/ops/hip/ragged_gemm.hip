@@ -36,6 +36,7 @@ enum { R_F32 = 0, R_F32_ACC = 1, R_BF16 = 2 };                // dW outputs
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 #define LDS_PTR(T, p) ((__attribute__((address_space(3))) T*)(p))
 
@@ -894,9 +895,36 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     const auto rd = __builtin_amdgcn_make_buffer_rsrc((char*)a.der + base * 2, (short)0, 0x7fffffff, 0x00027000);
     const int ncols = a.N - w.n0, nrows = KIND == R_TN ? a.M - w.m0 : w.rows;
     char* const turn_row = turn_lds[P_KC ? 0 : wave] + l15 * OUT_ROW;  // written by rows, 4 columns a lane
-    const char* const turn_at = turn_lds[P_KC ? 0 : wave] + g * OUT_ROW + l15 * 16;
+    char* const turn_at = turn_lds[P_KC ? 0 : wave] + g * OUT_ROW + l15 * 16;
+    // Slopes, or what sums are added to, of BATCH fragments at once: a load behind stores comes
+    // no earlier than these end (dx times slope, 256 experts of 1024 rows, 1024 -> 4096: 2607 us
+    // one by one, 2442 by 2, 2395 by 4, 2423 by 8).
+    constexpr bool ADDS = KIND == R_TN && EPI == R_F32_ACC;
+    constexpr int BATCH = ADDS ? 2 : 4;
+    f32x4 sums[ADDS ? BATCH : 1][2][4];
+    u32x4 slope[KIND == R_NN && EPI == R_MUL ? BATCH : 1][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
+      if (KIND == R_NN && EPI == R_MUL && j % BATCH == 0) {
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = (j + b) * 32 + wm * 16 + 4 * k + g, n = wn * 128 + l15 * 8;
+            const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
+            slope[b][k] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rd, off, 0, 0));
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (ADDS && j % BATCH == 0) {
+#pragma unroll
+        for (int b = 0; b < BATCH * 8; ++b) {
+          const int r = (j + b / 8) * 32 + wm * 16 + 4 * (b % 4) + g, n = wn * 128 + b / 4 % 2 * 64 + l15 * 4;
+          const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 4 : OOB_OFFSET;
+          sums[b / 8][b / 4 % 2][b % 4] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, off, 0, 0));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) pin_acc(acc[i][j]);
       const int r0 = j * 32 + wm * 16;
@@ -927,6 +955,11 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, d), rd, off, 0, STREAMED);
         }
       } else {
+        if (EPI == R_MUL && KIND == R_NN) {  // to where its products go
+#pragma unroll
+          for (int k = 0; k < 4; ++k) *(u32x4*)(turn_at + 4 * k * OUT_ROW) = slope[j % BATCH][k];
+          asm volatile("" ::: "memory");
+        }
 #pragma unroll
         for (int h = 0; h < (F32 ? 2 : 1); ++h) {  // 256 bytes: 64 numbers of 32 bits or 128 of 16
           if (F32) {
@@ -940,10 +973,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
 #pragma unroll
                 for (int x = 0; x < 4; ++x) o[x] = f2bf(acc[i][j][x]);
               } else {
-                typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
-                const int r = r0 + l15, n = wn * 128 + i * 16 + g * 4;
-                const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
-                const f16x4 d = __builtin_bit_cast(f16x4, __builtin_amdgcn_raw_buffer_load_b64(rd, off, 0, 0));
+                const f16x4 d = *(const f16x4*)(turn_row + (i * 16 + g * 4) * 2);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) o[x] = f2bf(acc[i][j][x] * (float)d[x]);
               }
@@ -962,8 +992,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
             const int r = r0 + 4 * k + g;
             const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * (F32 ? 4 : 2) : OOB_OFFSET;
             f32x4 v = turned[k];
-            if (KIND == R_TN && EPI == R_F32_ACC)
-              v += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, off, 0, 0));
+            if (ADDS) v += sums[j % BATCH][h][k];
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rc, off, 0, STREAMED);
           }
         }
