@@ -405,6 +405,7 @@ static void check_slope(const torch::Tensor& der) {
 
 static void check_weight(const torch::Tensor& w, const torch::Tensor& offsets) {
   TORCH_CHECK(w.dim() == 3 && w.size(0) == offsets.numel() - 1, "weight must be [E, N, K]");
+  TORCH_CHECK_VALUE(w.size(0) <= 4096, "at most 4096 experts, got ", w.size(0));  // the table of tiles
   TORCH_CHECK(w.size(1) > 0 && w.size(2) > 0 && w.size(1) % 8 == 0 && w.size(2) % 8 == 0,
               "N and K must be multiples of 8");
   TORCH_CHECK(w.size(1) * w.size(2) < (int64_t)1 << 30 && w.size(1) < 1 << 21 &&
@@ -433,10 +434,13 @@ std::vector<torch::Tensor> ragged_layout(torch::Tensor ids, int64_t E) {
 }
 
 // Tiles of 256 x 256 (one block a CU, a list of tiles) or 128 x 256: the large ones where
-// there is one for every CU and experts have rows for them. At 256 experts of 32 rows
-// 397 against 434 us, of 1024 rows 2377 against 2042 us (dx, 1024 <- 4096).
+// there are some for half the CUs and experts have rows for them. Large against small, us:
+// 8 experts of 512 rows, 1024 -> 1024 (64 tiles) 29 and 25, of 1024 rows (128) 31 and 38;
+// 256 experts, 1024 -> 4096, of 32 rows 405 and 452, of 64 rows 422 and 508; 4096 -> 1024, of
+// 64 rows 537 and 458, of 96 rows 522 and 550, of 256 rows 633 and 1071.
 static bool large_tiles(int64_t R, int64_t E, int64_t N) {
-  return R >= 128 * E && R / 256 * ((N + 255) / 256) >= 256;
+  const int64_t tiles = R / 256 * ((N + 255) / 256);
+  return (R >= 96 * E && tiles >= 128) || (R >= 64 * E && tiles >= 512);
 }
 
 static torch::Tensor tile_table(const torch::Tensor& rows, int64_t E, int64_t N) {

@@ -232,6 +232,7 @@ class TestGroupedLinear:
         (dict(bias=torch.zeros(2, 8)), "bias"),
         (dict(bias=torch.zeros(2, 16).half()), "bias"),
         (dict(activation="relu"), "activation"),
+        (dict(weight=torch.zeros(4097, 16, 8).bfloat16(), offsets=torch.zeros(4098).int()), "4096"),
     ])
     def test_refusals(self, change, match):
         args = dict(x=torch.zeros(4, 8).bfloat16(), weight=torch.zeros(2, 16, 8).bfloat16(),
@@ -287,6 +288,14 @@ class TestGroupedLinear:
     def test_weight_gradients_by_rows(self, counts):
         """More tiles than blocks, experts of very different rows."""
         p = problem(counts, 264, 776, tail=9)
+        want, tol = exact(*p, False)
+        got = run_all(*p, False)
+        for name in got:
+            close(name, got[name], want[name], tol[name])
+
+    @pytest.mark.parametrize("each", [1, 3, 100])
+    def test_most_experts(self, each):
+        p = problem([each] * 4096, 8, 136, tail=1)
         want, tol = exact(*p, False)
         got = run_all(*p, False)
         for name in got:
