@@ -414,7 +414,7 @@ __launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (single decoded tokens): each active expert's weight once through the CUs
+// Few rows (single decoded tokens, small products): an active expert's weight through the CUs
 //
 // Bound by HBM, or by latency. A block has 16 outputs of one expert for up to 16 of its
 // rows, its 4 waves a quarter of the contraction each; the weight goes from global memory
@@ -1151,12 +1151,16 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
 
-// 16-row tiles where experts have a row or none, or there are few rows at all. Of 256
+// 16-row tiles where experts have a row or none, or there are few rows at all: of 256
 // experts, 1024 -> 4096, 4 rows take 12 us so and 49 in 128-row tiles, 128 rows 158 and 168,
-// 1024 rows 422 and 361; of 4 experts 64 rows 15 and 22, 256 rows 41 and 23.
+// 1024 rows 422 and 361. And where 128-row tiles would leave most CUs idle, at a microsecond
+// for each 64 contraction steps, while the weights, read anew for every 16 rows, pass in
+// less: rows and experts by outputs decide, the contraction is in both. 4 experts of 64
+// rows, 1024 -> 1024 (20480): 12 and 21 us; 12 of 166, 136 -> 328 (44936): 8.0 and 8.3, with
+// the slope 8.6 and 11.3; 8 of 128, 256 -> 1024 (73728): 15 and 10.
 template <int EPI>
 static bool launch_few(const RaggedArgs& a, hipStream_t stream) {
-  if (a.R > a.E && a.R > 64) return false;
+  if (a.R > a.E && a.R > 64 && (a.R / FR + a.E) * a.N > 49152) return false;
   const long most = a.R < a.R / FR + a.E + 1 ? a.R : a.R / FR + a.E + 1;
   const int groups = cdiv(a.N, FR);
   // outputs a block, one group of 16 after the other: looking up its tile is as long as one

@@ -293,6 +293,29 @@ class TestGroupedLinear:
         for name in got:
             close(name, got[name], want[name], tol[name])
 
+    @pytest.mark.parametrize("counts", ["tiles", "skewed", "many"])
+    @pytest.mark.parametrize("K,N", [(264, 1288), (72, 2048), (8, 4096)])
+    @pytest.mark.parametrize("gelu", [False, True])
+    def test_wide_outputs(self, counts, K, N, gelu):
+        """Too many outputs for the small tiles, too few rows for the large ones."""
+        p = problem(COUNTS[counts], K, N, tail=5, bias=torch.bfloat16 if gelu else torch.float32)
+        want, tol = exact(*p, gelu)
+        got = run_all(*p, gelu)
+        for name in got:
+            close(name, got[name], want[name], tol[name])
+        with torch.no_grad():
+            y = Fops.grouped_linear(p[0], p[1], p[3], p[2], "gelu" if gelu else None)
+        close("y", y, want["y"], tol["y"])
+
+    def test_no_rows(self):
+        p = problem([0, 0, 0], 40, 24)
+        assert p[0].shape == (0, 40)
+        got = run_all(*p, True)
+        assert got["y"].shape == (0, 24) and got["dx"].shape == (0, 40)
+        assert not got["dw"].any() and not got["db"].any()
+        with torch.no_grad():
+            assert Fops.grouped_linear(p[0], p[1], p[3]).shape == (0, 24)
+
     @pytest.mark.parametrize("each", [1, 3, 100])
     def test_most_experts(self, each):
         p = problem([each] * 4096, 8, 136, tail=1)
