@@ -110,8 +110,13 @@ def _check_product(x, weight, offsets, bias, activation):
 def _check_gpu_product(x, weight):
     if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
         raise ValueError(f"the GPU kernels take bf16, got {x.dtype} and {weight.dtype}")
+    if weight.shape[0] == 0 or weight[0].numel() == 0:
+        raise ValueError(f"weight must not be empty, got {tuple(weight.shape)}")
     if weight.shape[1] % 8 or weight.shape[2] % 8:
         raise ValueError(f"N and K must be multiples of 8 (16-byte rows), got {tuple(weight.shape)}")
+    if weight[0].numel() >= 1 << 30 or max(weight.shape[1:]) >= 1 << 21:
+        raise ValueError(f"one expert's weight must have below 2^30 numbers, and N and K be below "
+                         f"2^21, got {tuple(weight.shape)}")
 
 
 def _ready(t: torch.Tensor) -> torch.Tensor:
