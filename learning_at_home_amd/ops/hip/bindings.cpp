@@ -45,9 +45,10 @@ long lah_ragged_layout_table(long, int);
 void lah_ragged_layout(const void*, int, long, int, void*, void*, void*, void*, hipStream_t);
 long lah_ragged_tiles_room(long, int);
 void lah_ragged_nt(const void*, const void*, void*, const void*, const void*, int, void*,
-                   long, int, int, int, int, void*, hipStream_t);
+                   long, int, int, int, int, void*, int, void*, hipStream_t);
 void lah_ragged_nn(const void*, const void*, void*, const void*, void*, long, int, int, int,
-                   void*, hipStream_t);
+                   void*, int, void*, hipStream_t);
+int lah_ragged_parts(long, int, int, int, bool);
 int lah_ragged_splits(long, int, int, int);
 long lah_ragged_order_room(long, int, int, int, int);
 void lah_ragged_tn(const void*, const void*, void*, void*, int, const void*, long, int, int,
@@ -448,6 +449,9 @@ static torch::Tensor tile_table(const torch::Tensor& rows, int64_t E, int64_t N)
   if (!large_tiles(R, E, N)) return {};
   return torch::empty({lah_ragged_tiles_room(R, (int)E) * 4}, rows.options().dtype(at::kInt));
 }
+static torch::Tensor part_sums(const torch::Tensor& rows, int parts, int64_t N) {
+  return parts > 1 ? torch::empty({parts * rows.size(0) * N}, rows.options().dtype(at::kFloat)) : torch::Tensor();
+}
 static void* ptr_or_null(const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // y[r] = act(W[e] x[r] + b[e]); epi 0 plain, 1 gelu, 2 gelu and its slope into der
@@ -480,8 +484,11 @@ torch::Tensor ragged_nt(torch::Tensor x, torch::Tensor w, torch::Tensor offsets,
   auto y = torch::empty({R, N}, x.options());
   if (R == 0) return y;
   const auto table = tile_table(x, E, N);
+  const int parts = table.defined() ? 1 : lah_ragged_parts(R, (int)E, (int)N, (int)K, true);
+  const auto work = part_sums(x, parts, N);
   lah_ragged_nt(x.data_ptr(), w.data_ptr(), y.data_ptr(), offsets.data_ptr(), bias_p, bias_bf16,
-                der_p, R, (int)E, (int)N, (int)K, (int)epi, ptr_or_null(table), cur_stream());
+                der_p, R, (int)E, (int)N, (int)K, (int)epi, ptr_or_null(table), parts,
+                ptr_or_null(work), cur_stream());
   CHECK_LAUNCH();
   return y;
 }
@@ -504,8 +511,10 @@ torch::Tensor ragged_nn(torch::Tensor d, torch::Tensor w, torch::Tensor offsets,
   auto out = torch::empty({R, N}, d.options());
   if (R == 0) return out;
   const auto table = tile_table(d, E, N);
+  const int parts = table.defined() ? 1 : lah_ragged_parts(R, (int)E, (int)N, (int)K, false);
+  const auto work = part_sums(d, parts, N);
   lah_ragged_nn(d.data_ptr(), w.data_ptr(), out.data_ptr(), offsets.data_ptr(), der_p, R, (int)E,
-                (int)N, (int)K, ptr_or_null(table), cur_stream());
+                (int)N, (int)K, ptr_or_null(table), parts, ptr_or_null(work), cur_stream());
   CHECK_LAUNCH();
   return out;
 }

@@ -32,7 +32,7 @@
 #define RT 256   // threads
 
 enum { R_NT = 0, R_NN = 1, R_TN = 2 };
-enum { R_PLAIN = 0, R_GELU = 1, R_GELU_DER = 2, R_MUL = 3 };  // forward epilogues
+enum { R_PLAIN = 0, R_GELU = 1, R_GELU_DER = 2, R_MUL = 3, R_PART = 4 };  // epilogues of rows; fp32 sums of a part
 enum { R_F32 = 0, R_F32_ACC = 1, R_BF16 = 2 };                // dW outputs
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
@@ -171,7 +171,7 @@ struct RaggedArgs {
   long R;
   int E, N, M, K;    // K: contraction of NT / NN
   int bias_bf16;     // of bias, or of db
-  int splits;        // TN: parts of each expert's rows, each with sums of its own
+  int splits;        // parts of the contraction, each with sums of its own
   bool once;         // weights that no cache holds until they are read again
 };
 
@@ -225,7 +225,9 @@ __launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
   const long row0 = lo + m0;
   if (q < 0 || size <= 0 || row0 >= hi || n0 >= a.N) return;  // also where offsets do not ascend
   const int rows = (int)min(hi - row0, (long)RBM);
-  const int steps = e == a.E ? 0 : cdiv(a.K, 64);
+  const int all = e == a.E ? 0 : cdiv(a.K, 64);
+  const int begin = EPI == R_PART ? all * (int)blockIdx.y / a.splits : 0;
+  const int steps = EPI == R_PART ? all * ((int)blockIdx.y + 1) / a.splits : all;  // the end
 
   // ---- staging: a thread's byte offsets in a tile are the same in every stage
   const __bf16* Pb = a.P + ((long)e * a.N * a.K + (P_KC ? (long)n0 * a.K : n0));
@@ -303,12 +305,12 @@ __launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
     return *(const bf16x8*)(smem + (p % 3) * SLOT + r * 64 + ((kk * 4 + g) ^ kc_swz<4>(r)) * 8);
   };
 
-  if (steps > 0) {
-    stage_p(0);
-    stage_q(0);
-    stage_p(1);
+  if (begin < steps) {
+    stage_p(2 * begin);
+    stage_q(begin);
+    stage_p(2 * begin + 1);
   }
-  for (int t = 0; t < steps; ++t) {
+  for (int t = begin; t < steps; ++t) {
     const bool more = t + 1 < steps;
     bf16x8 qf[4][2];
     // the phase's loads have landed; all waves are past their reads of what is refilled now
@@ -373,6 +375,12 @@ __launch_bounds__(RT, 2) __global__ void ragged_rows_kernel(RaggedArgs a) {
       float v[STEP];
 #pragma unroll
       for (int x = 0; x < STEP; ++x) v[x] = acc[i0 + x / 4][j][x & 3];
+      if (EPI == R_PART) {
+        float* to = (float*)a.C + ((long)blockIdx.y * a.R * a.N + at + n);
+#pragma unroll
+        for (int h = 0; h < STEP; h += 4) *(f32x4*)(to + h) = f32x4{v[h], v[h + 1], v[h + 2], v[h + 3]};
+        continue;
+      }
       if (KIND == R_NT && a.bias != nullptr && e < a.E) {
         if (a.bias_bf16) {
           const bf16x8 b = *(const bf16x8*)((const __bf16*)a.bias + (long)e * a.N + n);
@@ -1158,16 +1166,16 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
 // less: rows and experts by outputs decide, the contraction is in both. 4 experts of 64
 // rows, 1024 -> 1024 (20480): 12 and 21 us; 12 of 166, 136 -> 328 (44936): 8.0 and 8.3, with
 // the slope 8.6 and 11.3; 8 of 128, 256 -> 1024 (73728): 15 and 10.
+static bool few_rows(long R, int E, int N) { return R <= E || R <= 64 || (R / FR + E) * N <= 49152; }
+
 template <int EPI>
-static bool launch_few(const RaggedArgs& a, hipStream_t stream) {
-  if (a.R > a.E && a.R > 64 && (a.R / FR + a.E) * a.N > 49152) return false;
+static void launch_few(const RaggedArgs& a, hipStream_t stream) {
   const long most = a.R < a.R / FR + a.E + 1 ? a.R : a.R / FR + a.E + 1;
   const int groups = cdiv(a.N, FR);
   // outputs a block, one group of 16 after the other: looking up its tile is as long as one
   const int per = (int)(most * groups <= 8192 ? 1 : most * groups <= 32768 ? 4 : 8);
   hipLaunchKernelGGL((ragged_few_kernel<EPI>), dim3(cdiv(groups, per), (unsigned)most), dim3(256), 0, stream, a,
                      per);
-  return true;
 }
 
 // Weights larger than the last cache (256 MB) are gone before the next call, and where
@@ -1176,10 +1184,61 @@ static bool launch_few(const RaggedArgs& a, hipStream_t stream) {
 // its dx 346 and 383. Smaller weights lose by it: 64 of 1024 x 1024, 64 rows each, 42 and 39.
 static bool read_once(int E, int N, int K) { return (long)E * N * K * 2 > (256l << 20); }
 
+// Rows from the parts' sums, in the parts' order, and what else belongs to them
+template <int EPI>
+__launch_bounds__(256) __global__ void ragged_join_rows_kernel(RaggedArgs a, const float* __restrict__ part) {
+  const long n = a.R * a.N, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 v = *(const f32x4*)(part + i);
+  for (int p = 1; p < a.splits; ++p) v += *(const f32x4*)(part + p * n + i);
+  if (a.bias != nullptr) {
+    const long row = i / a.N;
+    int e = 0;  // the last group that starts at or before the row has it
+    for (int end = a.E; e < end;) {
+      const int mid = (e + end + 1) >> 1;
+      if (a.offsets[mid] <= row) e = mid;
+      else end = mid - 1;
+    }
+    if (e < a.E) {
+      const long at = (long)e * a.N + i % a.N;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        v[x] += a.bias_bf16 ? bf2f(((const __bf16*)a.bias)[at + x]) : ((const float*)a.bias)[at + x];
+    }
+  }
+  bf16x4 o;
+  f16x4 d;
+  if (EPI == R_MUL) d = *(const f16x4*)(a.der + i);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    if (EPI == R_GELU_DER) {
+      float y, s;
+      gelu_and_slope(v[x], &y, &s);
+      o[x] = f2bf(y);
+      d[x] = (_Float16)s;
+    } else {
+      o[x] = f2bf(EPI == R_GELU ? gelu_of(v[x]) : EPI == R_MUL ? v[x] * (float)d[x] : v[x]);
+    }
+  }
+  *(bf16x4*)((__bf16*)a.C + i) = o;
+  if (EPI == R_GELU_DER) *(f16x4*)(a.der + i) = d;
+}
+
+// Parts of the contraction where there are fewer tiles than CUs, a microsecond for each 64
+// steps; of few rows, whose sums are small, for two blocks a CU. 4 experts of 32 rows, dx
+// 1024 <- 4096: 77 us in one part, 20 in 12 and 25; 4 of 64 rows, 4096 -> 4096: 76, 47 in 2, 42
+// in 5; 8 of 512 rows, 1024 -> 1024, 29 us, 48 in 3 parts.
+extern "C" int lah_ragged_parts(long R, int E, int N, int K, bool forward) {
+  if (forward && few_rows(R, E, N)) return 1;
+  const long tiles = (R < R / RBM + E ? R : R / RBM + E) * ((N + RBN - 1) / RBN), most = (K + 63) / 64 / 4;
+  const long s = (R <= 512 ? 512 : 256) / (tiles < 1 ? 1 : tiles);
+  return (int)(s < most ? (s < 1 ? 1 : s) : most < 1 ? 1 : most);
+}
+
 template <int KIND, int EPI>
-static void launch_rows(const RaggedArgs& a, void* table, hipStream_t stream) {
+static void launch_rows(const RaggedArgs& a, void* table, void* work, hipStream_t stream) {
   if constexpr (KIND == R_NT)
-    if (launch_few<EPI>(a, stream)) return;
+    if (few_rows(a.R, a.E, a.N)) return launch_few<EPI>(a, stream);
   if (table != nullptr) {
     hipLaunchKernelGGL(ragged_tiles_kernel, dim3(1), dim3(1024), 0, stream, a.offsets, a.E, a.R, (int4*)table);
     const long most = (a.R / BM + a.E + 1) * ((a.N + BN - 1) / BN);
@@ -1187,8 +1246,16 @@ static void launch_rows(const RaggedArgs& a, void* table, hipStream_t stream) {
                        stream, a, (const int4*)table);
     return;
   }
-  const long tiles = (a.R / RBM + a.E + 1) * ((a.N + RBN - 1) / RBN);
-  hipLaunchKernelGGL((ragged_rows_kernel<KIND, EPI>), dim3((unsigned)tiles), dim3(RT), 0, stream, a);
+  const unsigned tiles = (unsigned)((a.R / RBM + a.E + 1) * ((a.N + RBN - 1) / RBN));
+  if (a.splits > 1) {
+    RaggedArgs part = a;
+    part.C = work;
+    hipLaunchKernelGGL((ragged_rows_kernel<KIND, R_PART>), dim3(tiles, a.splits), dim3(RT), 0, stream, part);
+    hipLaunchKernelGGL((ragged_join_rows_kernel<EPI>), dim3((unsigned)((a.R * a.N / 4 + 255) / 256)), dim3(256), 0,
+                       stream, a, (const float*)work);
+    return;
+  }
+  hipLaunchKernelGGL((ragged_rows_kernel<KIND, EPI>), dim3(tiles), dim3(RT), 0, stream, a);
 }
 
 // dW and db from the parts' sums, in the parts' order
@@ -1261,25 +1328,26 @@ extern "C" long lah_ragged_order_room(long R, int E, int N, int M, int splits) {
 // int4 entries a table of M-tiles needs
 extern "C" long lah_ragged_tiles_room(long R, int E) { return R / BM + E + 2; }
 
-// table: room for the M-tiles where the large tiles are to be used, or null
+// table: room for the M-tiles where the large tiles are to be used, or null. work: fp32 room for
+// parts * R * N, if there are more than one
 extern "C" void lah_ragged_nt(const void* x, const void* w, void* y, const void* offsets,
                               const void* bias, int bias_bf16, void* der, long R, int E, int N,
-                              int K, int epi, void* table, hipStream_t stream) {
+                              int K, int epi, void* table, int parts, void* work, hipStream_t stream) {
   RaggedArgs a{(const __bf16*)w, (const __bf16*)x, y, (const int*)offsets, bias, (_Float16*)der,
-               nullptr, R, E, N, 0, K, bias_bf16, 1, read_once(E, N, K)};
-  if (epi == R_GELU_DER) launch_rows<R_NT, R_GELU_DER>(a, table, stream);
-  else if (epi == R_GELU) launch_rows<R_NT, R_GELU>(a, table, stream);
-  else launch_rows<R_NT, R_PLAIN>(a, table, stream);
+               nullptr, R, E, N, 0, K, bias_bf16, parts, read_once(E, N, K)};
+  if (epi == R_GELU_DER) launch_rows<R_NT, R_GELU_DER>(a, table, work, stream);
+  else if (epi == R_GELU) launch_rows<R_NT, R_GELU>(a, table, work, stream);
+  else launch_rows<R_NT, R_PLAIN>(a, table, work, stream);
 }
 
 // dx[r] = W[e]^T d[r] (times der[r], if given): W [E, K, N], d [R, K], out [R, N]
 extern "C" void lah_ragged_nn(const void* d, const void* w, void* out, const void* offsets,
-                              void* der, long R, int E, int N, int K, void* table,
+                              void* der, long R, int E, int N, int K, void* table, int parts, void* work,
                               hipStream_t stream) {
   RaggedArgs a{(const __bf16*)w, (const __bf16*)d, out, (const int*)offsets, nullptr,
-               (_Float16*)der, nullptr, R, E, N, 0, K, 0, 1, read_once(E, N, K)};
-  if (der != nullptr) launch_rows<R_NN, R_MUL>(a, table, stream);
-  else launch_rows<R_NN, R_PLAIN>(a, table, stream);
+               (_Float16*)der, nullptr, R, E, N, 0, K, 0, parts, read_once(E, N, K)};
+  if (der != nullptr) launch_rows<R_NN, R_MUL>(a, table, work, stream);
+  else launch_rows<R_NN, R_PLAIN>(a, table, work, stream);
 }
 
 // Parts of each expert's rows, where there are fewer tiles than CUs and many rows to sum: at

@@ -26,7 +26,7 @@ def kernels(tmp_path_factory):
     for m in re.finditer(r"^(_Z\S*ragged_(?:big|rows)_kernel\S*):.*?\.Lfunc_end", text, re.M | re.S):
         lines = (line.split(";")[0].strip() for line in m.group(0).split("\n")[1:])
         found[m.group(1)] = [line for line in lines if line and not line.startswith(".") and not line.endswith(":")]
-    assert len(found) == 13
+    assert len(found) == 15
     return text, found
 
 
@@ -49,7 +49,7 @@ def slots(lines):
 def test_nothing_is_spilled(kernels):
     text, _ = kernels
     spills = re.findall(r"\.name:\s+(_Z\S*ragged_(?:big|rows)\S*).*?\.vgpr_spill_count:\s+(\d+)", text, re.S)
-    assert len(spills) == 13
+    assert len(spills) == 15
     assert {n for _, n in spills} == {"0"}
     assert not any(line.startswith("scratch_") for lines in kernels[1].values() for line in lines)
 

@@ -307,6 +307,55 @@ class TestGroupedLinear:
             y = Fops.grouped_linear(p[0], p[1], p[3], p[2], "gelu" if gelu else None)
         close("y", y, want["y"], tol["y"])
 
+    @pytest.mark.parametrize("counts", [[70, 0, 130, 1], [3, 0, 1], [600, 700]])
+    @pytest.mark.parametrize("K,N", [(1032, 2056), (2000, 1288), (4096, 1288), (1032, 136)])
+    @pytest.mark.parametrize("gelu", [False, True])
+    def test_contraction_in_parts(self, counts, K, N, gelu):
+        """Fewer tiles than CUs and a long contraction: summed in parts and joined."""
+        p = problem(counts, K, N, tail=7, bias=torch.bfloat16 if gelu else torch.float32)
+        want, tol = exact(*p, gelu)
+        got = run_all(*p, gelu)
+        for name in got:
+            close(name, got[name], want[name], tol[name])
+        again = run_all(*p, gelu)
+        for name in got:
+            assert torch.equal(got[name], again[name])
+        with torch.no_grad():
+            y = Fops.grouped_linear(p[0], p[1], p[3], p[2], "gelu" if gelu else None)
+        close("y", y, want["y"], tol["y"])
+
+    def test_parts_captured(self):
+        x, w, b, offsets, dy = problem([70, 0, 130, 1], 1032, 2056, tail=100)
+        leaves = [t.requires_grad_(True) for t in (x, w, b)]
+
+        def step():
+            y = Fops.grouped_linear(x, w, offsets, b, "gelu")
+            return (y, *torch.autograd.grad(y, leaves, dy))
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graphs = []
+        for _ in range(2):  # each with sums of its own
+            graphs.append((torch.cuda.CUDAGraph(), []))
+            with torch.cuda.graph(graphs[-1][0]):
+                graphs[-1][1].extend(step())
+        for counts in ([70, 0, 130, 1], [0, 301, 0, 0], [10, 20, 30, 40]):
+            with torch.no_grad():
+                offsets.copy_(offsets_of(counts))
+            torch.cuda.synchronize()
+            for graph, _ in graphs:
+                with torch.cuda.stream(side):
+                    graph.replay()
+                step()
+            torch.cuda.synchronize()
+            now = step()
+            for _, held in graphs:
+                for a, b_ in zip(held, now):
+                    assert torch.equal(a, b_)
+
     def test_no_rows(self):
         p = problem([0, 0, 0], 40, 24)
         assert p[0].shape == (0, 40)
