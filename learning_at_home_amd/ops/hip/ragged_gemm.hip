@@ -1159,14 +1159,17 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 }
 
-// 16-row tiles where experts have a row or none, or there are few rows at all: of 256
-// experts, 1024 -> 4096, 4 rows take 12 us so and 49 in 128-row tiles, 128 rows 158 and 168,
-// 1024 rows 422 and 361. And where 128-row tiles would leave most CUs idle, at a microsecond
-// for each 64 contraction steps, while the weights, read anew for every 16 rows, pass in
-// less: rows and experts by outputs decide, the contraction is in both. 4 experts of 64
-// rows, 1024 -> 1024 (20480): 12 and 21 us; 12 of 166, 136 -> 328 (44936): 8.0 and 8.3, with
-// the slope 8.6 and 11.3; 8 of 128, 256 -> 1024 (73728): 15 and 10.
-static bool few_rows(long R, int E, int N) { return R <= E || R <= 64 || (R / FR + E) * N <= 49152; }
+// 16-row tiles where experts have a row or none: of 256 experts, 1024 -> 4096, 4 rows take 12
+// us so and 49 in 128-row tiles, 128 rows 158 and 168, 1024 rows 422 and 361. And for small
+// products, which leave most CUs idle in 128-row tiles: by rows and experts times outputs (8
+// experts of 128 rows, 256 -> 256, 18432: 5.3 us and 10; 12 of 166, 136 -> 328, 44895: 8.2 and
+// 9.8; 8 of 128, 256 -> 1024, 73728: 15 and 10), as long as the weights, read anew for every
+// 16 rows, take no longer than a contraction in parts (4 of 64 rows, 1024 -> 1024, 21 million:
+// 12 and 15; 4 of 128, 38 million: 21 and 19; 4 of 16, 4096 -> 4096, 134 million: 41 and 28).
+static bool few_rows(long R, int E, int N, int K) {
+  const long outputs = (R / FR + E) * N;
+  return R <= E || (outputs <= 49152 && outputs * K <= 32 << 20);
+}
 
 template <int EPI>
 static void launch_few(const RaggedArgs& a, hipStream_t stream) {
@@ -1229,7 +1232,7 @@ __launch_bounds__(256) __global__ void ragged_join_rows_kernel(RaggedArgs a, con
 // 1024 <- 4096: 77 us in one part, 20 in 12 and 25; 4 of 64 rows, 4096 -> 4096: 76, 47 in 2, 42
 // in 5; 8 of 512 rows, 1024 -> 1024, 29 us, 48 in 3 parts.
 extern "C" int lah_ragged_parts(long R, int E, int N, int K, bool forward) {
-  if (forward && few_rows(R, E, N)) return 1;
+  if (forward && few_rows(R, E, N, K)) return 1;
   const long tiles = (R < R / RBM + E ? R : R / RBM + E) * ((N + RBN - 1) / RBN), most = (K + 63) / 64 / 4;
   const long s = (R <= 512 ? 512 : 256) / (tiles < 1 ? 1 : tiles);
   return (int)(s < most ? (s < 1 ? 1 : s) : most < 1 ? 1 : most);
@@ -1238,7 +1241,7 @@ extern "C" int lah_ragged_parts(long R, int E, int N, int K, bool forward) {
 template <int KIND, int EPI>
 static void launch_rows(const RaggedArgs& a, void* table, void* work, hipStream_t stream) {
   if constexpr (KIND == R_NT)
-    if (few_rows(a.R, a.E, a.N)) return launch_few<EPI>(a, stream);
+    if (few_rows(a.R, a.E, a.N, a.K)) return launch_few<EPI>(a, stream);
   if (table != nullptr) {
     hipLaunchKernelGGL(ragged_tiles_kernel, dim3(1), dim3(1024), 0, stream, a.offsets, a.E, a.R, (int4*)table);
     const long most = (a.R / BM + a.E + 1) * ((a.N + BN - 1) / BN);
