@@ -670,7 +670,7 @@ using number = std::integral_constant<int, N>;
 #define STREAMED 2   // stores do not stay in L2: dW of 1024 experts of 32 rows, 2048 x 512, 517 us -> 382
 
 struct BigTile {
-  int e, part = 0, rows, steps, m0, n0;
+  int e, part = 0, rows, steps, m0, n0, q;
   long row0;
 };
 
@@ -706,6 +706,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     }
     const int first = q / (4 * NT) * 4, size = min(MT - first, 4), in = q % (4 * NT);
     const int m = first + in % size;
+    w.q = q;
     w.n0 = in / size * BN;
     if (KIND == R_TN) {
       w.part = w.e / a.E;
@@ -729,6 +730,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     w.e = __builtin_amdgcn_readfirstlane(w.e);
     w.rows = __builtin_amdgcn_readfirstlane(w.rows);
     w.steps = __builtin_amdgcn_readfirstlane(w.steps);
+    w.q = __builtin_amdgcn_readfirstlane(w.q);
     w.row0 = (long)(unsigned)__builtin_amdgcn_readfirstlane((int)w.row0);
     return w;
   };
@@ -910,107 +912,120 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     const long base = (KIND == R_TN ? ((long)w.part * a.E + w.e) * a.M + w.m0 : w.row0) * a.N + w.n0;
     const auto rc = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + base * (F32 ? 4 : 2), (short)0, 0x7fffffff, 0x00027000);
     const auto rd = __builtin_amdgcn_make_buffer_rsrc((char*)a.der + base * 2, (short)0, 0x7fffffff, 0x00027000);
-    const int ncols = a.N - w.n0, nrows = KIND == R_TN ? a.M - w.m0 : w.rows;
-    char* const turn_row = turn_lds[P_KC ? 0 : wave] + l15 * OUT_ROW;  // written by rows, 4 columns a lane
-    char* const turn_at = turn_lds[P_KC ? 0 : wave] + g * OUT_ROW + l15 * 16;
-    // Slopes, or what sums are added to, of BATCH fragments at once: a load behind stores comes
-    // no earlier than these end (dx times slope, 256 experts of 1024 rows, 1024 -> 4096: 2607 us
-    // one by one, 2442 by 2, 2395 by 4, 2423 by 8).
-    constexpr bool ADDS = KIND == R_TN && EPI == R_F32_ACC;
-    constexpr int BATCH = ADDS ? 2 : 4;
-    f32x4 sums[ADDS ? BATCH : 1][2][4];
-    u32x4 slope[KIND == R_NN && EPI == R_MUL ? BATCH : 1][4];
+    const int ncols = a.N - w.n0, nrows = KIND != R_TN || (EPI == R_F32_ACC && w.rows == 0) ? w.rows : a.M - w.m0;
+    if (KIND == R_TN && EPI != R_F32_ACC && w.rows == 0) {
+      // No rows: the expert's zeros as they lie, whole lines whatever N is, as many stores as a
+      // tile has (186 experts of 2968 x 1392, 4 of them with rows: 591 us by tiles)
+      constexpr int CHUNK = BM * BN * (F32 ? 4 : 2);
+      const long size = (long)a.M * a.N * (F32 ? 4 : 2), from = (long)w.q * CHUNK;
+      const int here = (int)max(min(size - from, (long)CHUNK), 0l);
+      const auto rz = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + ((long)w.part * a.E + w.e) * size + from, (short)0,
+                                                        here, 0x00027000);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (KIND == R_NN && EPI == R_MUL && j % BATCH == 0) {
+      for (int i = 0; i < CHUNK / (BT * 16); ++i)
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{0, 0, 0, 0}, rz, (i * BT + wave * 64 + lane) * 16, 0, STREAMED);
+    } else {
+      char* const turn_row = turn_lds[P_KC ? 0 : wave] + l15 * OUT_ROW;  // written by rows, 4 columns a lane
+      char* const turn_at = turn_lds[P_KC ? 0 : wave] + g * OUT_ROW + l15 * 16;
+      // Slopes, or what sums are added to, of BATCH fragments at once: a load behind stores comes
+      // no earlier than these end (dx times slope, 256 experts of 1024 rows, 1024 -> 4096: 2607 us
+      // one by one, 2442 by 2, 2395 by 4, 2423 by 8).
+      constexpr bool ADDS = KIND == R_TN && EPI == R_F32_ACC;
+      constexpr int BATCH = ADDS ? 2 : 4;
+      f32x4 sums[ADDS ? BATCH : 1][2][4];
+      u32x4 slope[KIND == R_NN && EPI == R_MUL ? BATCH : 1][4];
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b)
+      for (int j = 0; j < 8; ++j) {
+        if (KIND == R_NN && EPI == R_MUL && j % BATCH == 0) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = (j + b) * 32 + wm * 16 + 4 * k + g, n = wn * 128 + l15 * 8;
-            const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
-            slope[b][k] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rd, off, 0, 0));
-          }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if (ADDS && j % BATCH == 0) {
+          for (int b = 0; b < BATCH; ++b)
 #pragma unroll
-        for (int b = 0; b < BATCH * 8; ++b) {
-          const int r = (j + b / 8) * 32 + wm * 16 + 4 * (b % 4) + g, n = wn * 128 + b / 4 % 2 * 64 + l15 * 4;
-          const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 4 : OOB_OFFSET;
-          sums[b / 8][b / 4 % 2][b % 4] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, off, 0, 0));
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) pin_acc(acc[i][j]);
-      const int r0 = j * 32 + wm * 16;
-      if (P_KC) {
-        const int n = wn * 128 + l15 * 8;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int r = r0 + 4 * g + x;
-          const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
-          bf16x8 o;
-          f16x8 d;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float v = acc[i][j][x];
-            if (EPI == R_GELU) {
-              o[i] = f2bf(gelu_of(v));
-            } else if (EPI == R_GELU_DER) {
-              float y, s;
-              gelu_and_slope(v, &y, &s);
-              o[i] = f2bf(y);
-              d[i] = (_Float16)s;
-            } else {
-              o[i] = f2bf(v);
+            for (int k = 0; k < 4; ++k) {
+              const int r = (j + b) * 32 + wm * 16 + 4 * k + g, n = wn * 128 + l15 * 8;
+              const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
+              slope[b][k] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rd, off, 0, 0));
             }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (ADDS && j % BATCH == 0) {
+#pragma unroll
+          for (int b = 0; b < BATCH * 8; ++b) {
+            const int r = (j + b / 8) * 32 + wm * 16 + 4 * (b % 4) + g, n = wn * 128 + b / 4 % 2 * 64 + l15 * 4;
+            const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 4 : OOB_OFFSET;
+            sums[b / 8][b / 4 % 2][b % 4] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, off, 0, 0));
           }
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rc, off, 0, STREAMED);
-          if (EPI == R_GELU_DER)
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, d), rd, off, 0, STREAMED);
-        }
-      } else {
-        if (EPI == R_MUL && KIND == R_NN) {  // to where its products go
-#pragma unroll
-          for (int k = 0; k < 4; ++k) *(u32x4*)(turn_at + 4 * k * OUT_ROW) = slope[j % BATCH][k];
-          asm volatile("" ::: "memory");
+          __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int h = 0; h < (F32 ? 2 : 1); ++h) {  // 256 bytes: 64 numbers of 32 bits or 128 of 16
-          if (F32) {
+        for (int i = 0; i < 8; ++i) pin_acc(acc[i][j]);
+        const int r0 = j * 32 + wm * 16;
+        if (P_KC) {
+          const int n = wn * 128 + l15 * 8;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) *(f32x4*)(turn_row + (i * 16 + g * 4) * 4) = acc[4 * h + i][j];
-          } else {
+          for (int x = 0; x < 4; ++x) {
+            const int r = r0 + 4 * g + x;
+            const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
+            bf16x8 o;
+            f16x8 d;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              bf16x4 o;
-              if (EPI != R_MUL) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[x] = f2bf(acc[i][j][x]);
+              const float v = acc[i][j][x];
+              if (EPI == R_GELU) {
+                o[i] = f2bf(gelu_of(v));
+              } else if (EPI == R_GELU_DER) {
+                float y, s;
+                gelu_and_slope(v, &y, &s);
+                o[i] = f2bf(y);
+                d[i] = (_Float16)s;
               } else {
-                const f16x4 d = *(const f16x4*)(turn_row + (i * 16 + g * 4) * 2);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[x] = f2bf(acc[i][j][x] * (float)d[x]);
+                o[i] = f2bf(v);
               }
-              *(bf16x4*)(turn_row + (i * 16 + g * 4) * 2) = o;
             }
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rc, off, 0, STREAMED);
+            if (EPI == R_GELU_DER)
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, d), rd, off, 0, STREAMED);
           }
-          const int n = wn * 128 + h * 64 + l15 * (F32 ? 4 : 8);
-          f32x4 turned[4];
-          // LDS works in the order of a wave's instructions; the compiler, who sees one lane, is to keep it
-          asm volatile("" ::: "memory");
+        } else {
+          if (EPI == R_MUL && KIND == R_NN) {  // to where its products go
 #pragma unroll
-          for (int k = 0; k < 4; ++k) turned[k] = *(const f32x4*)(turn_at + 4 * k * OUT_ROW);
-          asm volatile("" ::: "memory");
+            for (int k = 0; k < 4; ++k) *(u32x4*)(turn_at + 4 * k * OUT_ROW) = slope[j % BATCH][k];
+            asm volatile("" ::: "memory");
+          }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = r0 + 4 * k + g;
-            const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * (F32 ? 4 : 2) : OOB_OFFSET;
-            f32x4 v = turned[k];
-            if (ADDS) v += sums[j % BATCH][h][k];
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rc, off, 0, STREAMED);
+          for (int h = 0; h < (F32 ? 2 : 1); ++h) {  // 256 bytes: 64 numbers of 32 bits or 128 of 16
+            if (F32) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) *(f32x4*)(turn_row + (i * 16 + g * 4) * 4) = acc[4 * h + i][j];
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                bf16x4 o;
+                if (EPI != R_MUL) {
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) o[x] = f2bf(acc[i][j][x]);
+                } else {
+                  const f16x4 d = *(const f16x4*)(turn_row + (i * 16 + g * 4) * 2);
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) o[x] = f2bf(acc[i][j][x] * (float)d[x]);
+                }
+                *(bf16x4*)(turn_row + (i * 16 + g * 4) * 2) = o;
+              }
+            }
+            const int n = wn * 128 + h * 64 + l15 * (F32 ? 4 : 8);
+            f32x4 turned[4];
+            // LDS works in the order of a wave's instructions; the compiler, who sees one lane, is to keep it
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < 4; ++k) turned[k] = *(const f32x4*)(turn_at + 4 * k * OUT_ROW);
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int r = r0 + 4 * k + g;
+              const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * (F32 ? 4 : 2) : OOB_OFFSET;
+              f32x4 v = turned[k];
+              if (ADDS) v += sums[j % BATCH][h][k];
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rc, off, 0, STREAMED);
+            }
           }
         }
       }
