@@ -667,7 +667,21 @@ template <int N>
 using number = std::integral_constant<int, N>;
 
 #define OUT_ROW 272  // bytes
-#define STREAMED 2   // stores do not stay in L2: dW of 1024 experts of 32 rows, 2048 x 512, 517 us -> 382
+
+// Stores of whole lines need not stay in L2, parts of lines meet there: dW of 1024 experts of
+// 32 rows, 2048 x 512, 382 us and 517 where they stay, of 300 of 32 rows, 2936 x 1400, 886 and 655.
+template <typename T, typename Rsrc>
+LAH_DEVINL void store4(const T (&v)[4], Rsrc to, const unsigned (&off)[4], bool lines) {
+  if (lines) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), to, off[k], 0, 2);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[k]), to, off[k], 0, 0);
+  }
+}
 
 struct BigTile {
   int e, part = 0, rows, steps, m0, n0, q;
@@ -912,6 +926,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     const long base = (KIND == R_TN ? ((long)w.part * a.E + w.e) * a.M + w.m0 : w.row0) * a.N + w.n0;
     const auto rc = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + base * (F32 ? 4 : 2), (short)0, 0x7fffffff, 0x00027000);
     const auto rd = __builtin_amdgcn_make_buffer_rsrc((char*)a.der + base * 2, (short)0, 0x7fffffff, 0x00027000);
+    const bool lines = (a.N * (F32 ? 4 : 2)) % 128 == 0;
     const int ncols = a.N - w.n0, nrows = KIND != R_TN || (EPI == R_F32_ACC && w.rows == 0) ? w.rows : a.M - w.m0;
     if (KIND == R_TN && EPI != R_F32_ACC && w.rows == 0) {
       // No rows: the expert's zeros as they lie, whole lines whatever N is, as many stores as a
@@ -923,7 +938,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
                                                         here, 0x00027000);
 #pragma unroll
       for (int i = 0; i < CHUNK / (BT * 16); ++i)
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4{0, 0, 0, 0}, rz, (i * BT + wave * 64 + lane) * 16, 0, STREAMED);
+        __builtin_amdgcn_raw_buffer_store_b128(u32x4{0, 0, 0, 0}, rz, (i * BT + wave * 64 + lane) * 16, 0, 2);
     } else {
       char* const turn_row = turn_lds[P_KC ? 0 : wave] + l15 * OUT_ROW;  // written by rows, 4 columns a lane
       char* const turn_at = turn_lds[P_KC ? 0 : wave] + g * OUT_ROW + l15 * 16;
@@ -961,30 +976,30 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
         const int r0 = j * 32 + wm * 16;
         if (P_KC) {
           const int n = wn * 128 + l15 * 8;
+          unsigned off[4];
+          bf16x8 o[4];
+          f16x8 d[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int r = r0 + 4 * g + x;
-            const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
-            bf16x8 o;
-            f16x8 d;
+            off[x] = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * 2 : OOB_OFFSET;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float v = acc[i][j][x];
               if (EPI == R_GELU) {
-                o[i] = f2bf(gelu_of(v));
+                o[x][i] = f2bf(gelu_of(v));
               } else if (EPI == R_GELU_DER) {
                 float y, s;
                 gelu_and_slope(v, &y, &s);
-                o[i] = f2bf(y);
-                d[i] = (_Float16)s;
+                o[x][i] = f2bf(y);
+                d[x][i] = (_Float16)s;
               } else {
-                o[i] = f2bf(v);
+                o[x][i] = f2bf(v);
               }
             }
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), rc, off, 0, STREAMED);
-            if (EPI == R_GELU_DER)
-              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, d), rd, off, 0, STREAMED);
           }
+          store4(o, rc, off, lines);
+          if (EPI == R_GELU_DER) store4(d, rd, off, lines);
         } else {
           if (EPI == R_MUL && KIND == R_NN) {  // to where its products go
 #pragma unroll
@@ -1018,14 +1033,14 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
 #pragma unroll
             for (int k = 0; k < 4; ++k) turned[k] = *(const f32x4*)(turn_at + 4 * k * OUT_ROW);
             asm volatile("" ::: "memory");
+            unsigned off[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const int r = r0 + 4 * k + g;
-              const unsigned off = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * (F32 ? 4 : 2) : OOB_OFFSET;
-              f32x4 v = turned[k];
-              if (ADDS) v += sums[j % BATCH][h][k];
-              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rc, off, 0, STREAMED);
+              off[k] = r < nrows && n < ncols ? (unsigned)(r * a.N + n) * (F32 ? 4 : 2) : OOB_OFFSET;
+              if (ADDS) turned[k] += sums[j % BATCH][h][k];
             }
+            store4(turned, rc, off, lines);
           }
         }
       }
