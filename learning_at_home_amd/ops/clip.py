@@ -78,15 +78,16 @@ def master_sgd_step_(params: Sequence[torch.Tensor], masters: Sequence[torch.Ten
         raise ValueError("momentum needs momentum_bufs")
     if not params:
         return
-    if any(m.dtype != torch.float32 for m in masters + bufs):
-        raise ValueError("masters and momentum_bufs must be fp32")
-    if any(p.shape != m.shape or p.shape != g.shape for p, m, g in zip(params, masters, grads)):
-        raise ValueError("params, masters and grads must have the same shapes")
-    if any(p.shape != b.shape for p, b in zip(params, bufs)):
-        raise ValueError("momentum_bufs must have the shapes of the params")
-    if HAS_HIP and params[0].is_cuda:
+    if HAS_HIP and params[0].is_cuda:  # with the same checks
         if _C.master_sgd_(params, masters, grads, bufs, grad_scale, lr, momentum, weight_decay):
             return
+    else:
+        if any(m.dtype != torch.float32 for m in masters + bufs):
+            raise ValueError("masters and momentum_bufs must be fp32")
+        if any(p.shape != m.shape or p.shape != g.shape for p, m, g in zip(params, masters, grads)):
+            raise ValueError("params, masters and grads must have the same shapes")
+        if any(p.shape != b.shape for p, b in zip(params, bufs)):
+            raise ValueError("momentum_bufs must have the shapes of the params")
     for i in range(len(params)):
         b = bufs[i : i + 1]
         if HAS_HIP and params[i].is_cuda and _C.master_sgd_(params[i : i + 1], masters[i : i + 1], grads[i : i + 1],

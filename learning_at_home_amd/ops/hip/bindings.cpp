@@ -706,22 +706,28 @@ bool grad_scale_(const std::vector<torch::Tensor>& grads, const torch::Tensor& s
 bool master_sgd_(const std::vector<torch::Tensor>& params, const std::vector<torch::Tensor>& masters,
                  const std::vector<torch::Tensor>& grads, const std::vector<torch::Tensor>& bufs,
                  const c10::optional<torch::Tensor>& scale, double lr, double mu, double weight_decay) {
+  const size_t count = params.size();
+  TORCH_CHECK_VALUE(masters.size() == count && grads.size() == count && (bufs.empty() || bufs.size() == count),
+                    "params, masters, grads and momentum_bufs must go together");
+  for (size_t i = 0; i < count; ++i) {
+    TORCH_CHECK_VALUE(masters[i].scalar_type() == at::kFloat &&
+                      (bufs.empty() || bufs[i].scalar_type() == at::kFloat),
+                      "masters and momentum_bufs must be fp32");
+    TORCH_CHECK_VALUE(params[i].sizes() == masters[i].sizes() && params[i].sizes() == grads[i].sizes(),
+                      "params, masters and grads must have the same shapes");
+    TORCH_CHECK_VALUE(bufs.empty() || bufs[i].sizes() == params[i].sizes(),
+                      "momentum_bufs must have the shapes of the params");
+  }
   const ClipList p(params), m(masters), g(grads);
-  bool taken = p.taken && m.taken && g.taken;
-  TORCH_CHECK_VALUE(p.n == m.n && p.n == g.n, "params, masters and grads must have the same shapes");
-  TORCH_CHECK_VALUE(params[0].device() == masters[0].device() && params[0].device() == grads[0].device(),
-                    "all tensors must be on one device");
+  bool taken = p.taken && m.taken && g.taken && masters[0].device() == params[0].device() &&
+               grads[0].device() == params[0].device();
   std::vector<void*> b;
   if (!bufs.empty()) {
     const ClipList l(bufs);
-    TORCH_CHECK_VALUE(l.n == p.n, "momentum_bufs must have the shapes of the params");
-    TORCH_CHECK_VALUE(bufs[0].device() == params[0].device(), "all tensors must be on one device");
-    taken = taken && l.taken;
-    for (const int k : l.kind) taken = taken && k == 2;
+    taken = taken && l.taken && bufs[0].device() == params[0].device();
     b = l.p;
   }
   for (const int k : p.kind) taken = taken && k == 0;
-  for (const int k : m.kind) taken = taken && k == 2;
   if (!taken) return false;
   const void* s = scale_ptr(scale, params[0]);
   ON_DEVICE_OF(params[0]);

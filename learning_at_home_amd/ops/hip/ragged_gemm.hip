@@ -1383,11 +1383,14 @@ extern "C" void lah_ragged_nn(const void* d, const void* w, void* out, const voi
   else launch_rows<R_NN, R_PLAIN>(a, table, work, stream);
 }
 
-// Parts of each expert's rows, where there are fewer tiles than CUs and many rows to sum: at
-// least 4 stages a part. 16 experts of 1024 rows, 512 x 512: 93 us in one part, 48 in four.
+// Parts of each expert's rows, where there are fewer tiles than CUs: tiles for all of them, or
+// for each twice where there are many, since experts' rows are not alike; at least 4 stages a
+// part in the mean. 2 experts of 131072 rows, 512 x 512 (8 tiles): 2655 us in one part, 146 in
+// 32, 221 in 64; 8 with 13123 of 32768 rows, 1024 x 1024 (128 tiles), 272 in one, 160 in 2, 117
+// in 4, 171 in 8; 16 of 1024 rows, 512 x 512, 31 in one and 37 in 4.
 extern "C" int lah_ragged_splits(long R, int E, int N, int M) {
   const long tiles = weight_tiles(E, N, M), most = R / E / 256;
-  const long s = tiles < 256 ? 256 / tiles : 1;
+  const long s = tiles < 64 ? 256 / tiles : tiles < 256 ? 512 / tiles : 1;
   return (int)(s < most ? s : most < 1 ? 1 : most);
 }
 
