@@ -49,10 +49,9 @@ void lah_ragged_nt(const void*, const void*, void*, const void*, const void*, in
 void lah_ragged_nn(const void*, const void*, void*, const void*, void*, long, int, int, int,
                    void*, int, void*, hipStream_t);
 int lah_ragged_parts(long, int, int, int, bool);
-int lah_ragged_splits(long, int, int, int);
-long lah_ragged_order_room(long, int, int, int, int);
+long lah_ragged_tn_work(long, int, int, int);
 void lah_ragged_tn(const void*, const void*, void*, void*, int, const void*, long, int, int,
-                   int, int, int, void*, hipStream_t);
+                   int, int, void*, hipStream_t);
 void lah_ragged_slope(const void*, const void*, void*, long, hipStream_t);
 long lah_clip_partials(int);
 void lah_grad_norm(void* const*, const long*, const int*, int, void*, float, float, void*,
@@ -545,13 +544,11 @@ void ragged_tn(torch::Tensor d, torch::Tensor x, torch::Tensor offsets, torch::T
     db_p = db->data_ptr();
   }
   ON_DEVICE_OF(d);
-  const int splits = lah_ragged_splits(R, (int)E, (int)N, (int)M);
-  const long order = lah_ragged_order_room(R, (int)E, (int)N, (int)M, splits);
+  const long bytes = lah_ragged_tn_work(R, (int)E, (int)N, (int)M);
   torch::Tensor work;
-  if (splits > 1) work = torch::empty({splits * E * M * (N + 1)}, d.options().dtype(at::kFloat));
-  else if (order > 0) work = torch::empty({order}, d.options().dtype(at::kInt));
+  if (bytes > 0) work = torch::empty({bytes / 4}, d.options().dtype(at::kInt));
   lah_ragged_tn(d.data_ptr(), x.data_ptr(), dw.data_ptr(), db_p, db_bf16, offsets.data_ptr(), R,
-                (int)E, (int)N, (int)M, bf16 ? 2 : accumulate ? 1 : 0, splits, ptr_or_null(work),
+                (int)E, (int)N, (int)M, bf16 ? 2 : accumulate ? 1 : 0, ptr_or_null(work),
                 cur_stream());
   CHECK_LAUNCH();
 }

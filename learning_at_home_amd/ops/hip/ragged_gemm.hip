@@ -684,7 +684,7 @@ LAH_DEVINL void store4(const T (&v)[4], Rsrc to, const unsigned (&off)[4], bool 
 }
 
 struct BigTile {
-  int e, part = 0, rows, steps, m0, n0, q;
+  int e, out = 0, rows, steps, m0, n0, q;  // out: dW's place
   long row0;
 };
 
@@ -702,7 +702,8 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
   const int NT = cdiv(a.N, BN);
   // M-tiles of one expert, or of all
   const int MT = KIND == R_TN ? cdiv(a.M, BM) : __builtin_amdgcn_readfirstlane(table[0].x);
-  const int tiles = KIND == R_TN ? a.splits * a.E * MT * NT : MT * NT;
+  const int groups = KIND != R_TN ? 1 : table == nullptr ? a.splits * a.E : __builtin_amdgcn_readfirstlane(table[0].x);
+  const int tiles = groups * MT * NT;
   // 32 neighbouring tiles at a time on the 32 CUs of an XCD (blocks go to XCDs in turn)
   const int stride = gridDim.x;
   const int mine = stride % 256 == 0 ? (blockIdx.x & ~255) | ((blockIdx.x & 7) << 5) | ((blockIdx.x >> 3) & 31)
@@ -723,14 +724,22 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     w.q = q;
     w.n0 = in / size * BN;
     if (KIND == R_TN) {
-      w.part = w.e / a.E;
-      w.e -= w.part * a.E;
-      if (table != nullptr) w.e = ((const int*)table)[w.e];  // experts of many rows first
-      long lo, hi;
-      expert_rows(a, w.e, &lo, &hi);
-      const long each = a.splits == 1 ? hi - lo : (((hi - lo) / a.splits + 64) & ~63L);
-      w.row0 = min(lo + w.part * each, hi);
-      w.rows = (int)min(each, hi - w.row0);
+      if (table != nullptr) {
+        const int4 t = table[1 + w.e];
+        w.e = t.x;
+        w.row0 = t.y;
+        w.rows = t.z;
+        w.out = t.w;
+      } else {  // parts of equal rows
+        w.out = w.e;
+        const int part = w.e / a.E;
+        w.e -= part * a.E;
+        long lo, hi;
+        expert_rows(a, w.e, &lo, &hi);
+        const long each = a.splits == 1 ? hi - lo : (((hi - lo) / a.splits + 64) & ~63L);
+        w.row0 = min(lo + part * each, hi);
+        w.rows = (int)min(each, hi - w.row0);
+      }
       w.m0 = m * BM;
       w.steps = max(cdiv(w.rows, 64), 1);
     } else {
@@ -745,6 +754,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     w.rows = __builtin_amdgcn_readfirstlane(w.rows);
     w.steps = __builtin_amdgcn_readfirstlane(w.steps);
     w.q = __builtin_amdgcn_readfirstlane(w.q);
+    w.out = __builtin_amdgcn_readfirstlane(w.out);
     w.row0 = (long)(unsigned)__builtin_amdgcn_readfirstlane((int)w.row0);
     return w;
   };
@@ -923,7 +933,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
     int l15 = lane & 15, g = lane >> 4;
     asm volatile("" : "+v"(l15), "+v"(g));  // offsets made from these are not kept through the loop
     settle();
-    const long base = (KIND == R_TN ? ((long)w.part * a.E + w.e) * a.M + w.m0 : w.row0) * a.N + w.n0;
+    const long base = (KIND == R_TN ? (long)w.out * a.M + w.m0 : w.row0) * a.N + w.n0;
     const auto rc = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + base * (F32 ? 4 : 2), (short)0, 0x7fffffff, 0x00027000);
     const auto rd = __builtin_amdgcn_make_buffer_rsrc((char*)a.der + base * 2, (short)0, 0x7fffffff, 0x00027000);
     const bool lines = (a.N * (F32 ? 4 : 2)) % 128 == 0;
@@ -934,7 +944,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
       constexpr int CHUNK = BM * BN * (F32 ? 4 : 2);
       const long size = (long)a.M * a.N * (F32 ? 4 : 2), from = (long)w.q * CHUNK;
       const int here = (int)max(min(size - from, (long)CHUNK), 0l);
-      const auto rz = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + ((long)w.part * a.E + w.e) * size + from, (short)0,
+      const auto rz = __builtin_amdgcn_make_buffer_rsrc((char*)a.C + w.out * size + from, (short)0,
                                                         here, 0x00027000);
 #pragma unroll
       for (int i = 0; i < CHUNK / (BT * 16); ++i)
@@ -1051,7 +1061,7 @@ __launch_bounds__(BT, 1) __global__ void ragged_big_kernel(RaggedArgs a, const i
         pin_vgpr(dbacc[x]);
         const int m = w.m0 + (4 * wn + x) * 32 + wm * 16 + l15;
         if (m < a.M) {
-          const long at = ((long)w.part * a.E + w.e) * a.M + m;
+          const long at = (long)w.out * a.M + m;
           if (a.bias_bf16) ((__bf16*)a.db)[at] = f2bf(dbacc[x][0]);
           else ((float*)a.db)[at] = (EPI == R_F32_ACC ? ((float*)a.db)[at] : 0.f) + dbacc[x][0];
         }
@@ -1320,10 +1330,10 @@ static void join(const float* part, int splits, long n, void* out, int kind, hip
 static long weight_tiles(int E, int N, int M) { return (long)E * ((M + BM - 1) / BM) * ((N + BN - 1) / BN); }
 
 template <int OUT>
-static void launch_weights(const RaggedArgs& a, const int* order, hipStream_t stream) {
+static void launch_weights(const RaggedArgs& a, const int4* table, hipStream_t stream) {
   const long tiles = a.splits * weight_tiles(a.E, a.N, a.M);
   hipLaunchKernelGGL((ragged_big_kernel<R_TN, OUT>), dim3((unsigned)(tiles < 256 ? tiles : 256)), dim3(BT), 0,
-                     stream, a, (const int4*)order);
+                     stream, a, table);
 }
 
 // order[i] = the expert with the i'th most rows, the lower one of two as large
@@ -1349,15 +1359,104 @@ __launch_bounds__(256) __global__ void ragged_order_kernel(const int* __restrict
   order[rank] = mine;
 }
 
-// Numbers an order of the experts takes; 0 where the tiles come as they are. Tiles are as
-// long as their expert's rows, and a block has every 256th. 256 experts with 15358 rows down
-// to none, 262144 in all, 4096 x 1024: 2403 us in the experts' order, 2254 back and forth,
-// 2167 by rows. Few rows are bound by the stores, which the longer tiles' products then no
-// longer hide: 1024 experts, 32768 rows, 1280 down to none, 512 x 2048: 404 and 450.
-extern "C" long lah_ragged_order_room(long R, int E, int N, int M, int splits) {
-  return splits == 1 && E > 1 && E <= ORDERED && R / 256 >= E && weight_tiles(E, N, M) > 256 ? E : 0;
+// Lists for experts with very different rows. Tiles are as long as their expert's rows, L of
+// which are half of what a CU has to do in all. Experts of more than that come first, in pieces
+// of L with sums of their own, where the largest has over 4 L; else those of more than 2 L; the
+// others come whole and by their rows: pieces[0] = {number, experts}, pieces[1 + i] = {expert, first row,
+// rows, i}, joins[k] = {expert, its first piece, pieces}; whole[0] = {number}, whole[1 + i] =
+// {expert, first row, rows, expert}.
+__launch_bounds__(1024) __global__ void ragged_pieces_kernel(const int* __restrict__ offsets, int E, long R, long L,
+                                                             int room, const int* __restrict__ order,
+                                                             int4* __restrict__ pieces, int4* __restrict__ joins,
+                                                             int4* __restrict__ whole) {
+  __shared__ int wsum[16][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int PER = ORDERED / 1024;
+  int es[PER], c[PER], at = 0, large = 0;
+  long lo[PER], rows[PER];
+  const int e0 = order[0];
+  const long lo0 = e0 == 0 ? 0 : min((long)max(offsets[e0], 0), R);
+  const long whole_rows = min(max((long)offsets[e0 + 1], lo0), R) - lo0 > 4 * L ? L : 2 * L;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = tid * PER + j;
+    c[j] = 0;
+    if (i >= E) continue;
+    es[j] = order[i];
+    lo[j] = es[j] == 0 ? 0 : min((long)max(offsets[es[j]], 0), R);
+    rows[j] = min(max((long)offsets[es[j] + 1], lo[j]), R) - lo[j];
+    if (rows[j] > whole_rows) c[j] = (int)((rows[j] + L - 1) / L);
+    at += c[j];
+    large += c[j] > 0;
+  }
+  int inc = at, linc = large;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(inc, d, 64), u = __shfl_up(linc, d, 64);
+    if (lane >= d) inc += v, linc += u;
+  }
+  if (lane == 63) wsum[wave][0] = inc, wsum[wave][1] = linc;
+  __syncthreads();
+  int first = inc - at, total = 0, most = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    first += w < wave ? wsum[w][0] : 0;
+    total += wsum[w][0];
+    most += wsum[w][1];
+  }
+  if (tid == 0) {
+    pieces[0] = make_int4(min(total, room), most, 0, 0);
+    whole[0] = make_int4(E - most, 0, 0, 0);
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = tid * PER + j;
+    if (i >= E) continue;
+    if (c[j] == 0) {  // by rows: the large ones are in front
+      whole[1 + i - most] = make_int4(es[j], (int)lo[j], (int)rows[j], es[j]);
+      continue;
+    }
+    // more pieces than there is room for: only where offsets do not ascend
+    const int n = max(min(c[j], room - first), 0);
+    if (i < room) joins[i] = make_int4(es[j], first, n, 0);
+    for (int p = 0; p < n; ++p)
+      pieces[1 + first + p] = make_int4(es[j], (int)(lo[j] + p * L), (int)min(rows[j] - p * L, L), first + p);
+    first += c[j];
+  }
 }
 
+// dW and db of the experts in pieces, from the pieces' sums, in order
+template <int OUT>
+__launch_bounds__(256) __global__ void ragged_join_pieces_kernel(RaggedArgs a, const int4* __restrict__ pieces,
+                                                                 const int4* __restrict__ joins, int room,
+                                                                 const float* __restrict__ part) {
+  if ((int)blockIdx.y >= pieces[0].y) return;
+  const int4 t = joins[blockIdx.y];
+  const long n = (long)a.M * a.N, i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n + (a.db != nullptr ? a.M : 0) || t.z == 0) return;
+  const bool is_db = i >= n;
+  const float* from = is_db ? part + room * n + (long)t.y * a.M + (i - n) : part + t.y * n + i;
+  f32x4 sum = *(const f32x4*)from;
+  for (int p = 1; p < t.z; ++p) sum += *(const f32x4*)(from + p * (is_db ? a.M : n));
+  if (is_db ? a.bias_bf16 != 0 : OUT == R_BF16) {
+    bf16x4 o;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) o[x] = f2bf(sum[x]);
+    *(bf16x4*)(is_db ? (__bf16*)a.db + (long)t.x * a.M + (i - n) : (__bf16*)a.C + t.x * n + i) = o;
+  } else {
+    float* c = is_db ? (float*)a.db + (long)t.x * a.M + (i - n) : (float*)a.C + t.x * n + i;
+    *(f32x4*)c = OUT == R_F32_ACC ? *(const f32x4*)c + sum : sum;
+  }
+}
+
+// The work of dW, in bytes: sums of parts (splits > 1), or lists and sums of pieces
+// (where L > 0), or nothing.
+struct WeightWork {
+  int splits;
+  long L;     // rows a piece
+  int room;   // pieces at most
+  long bytes, sums;  // in all; where the sums begin
+};
 // int4 entries a table of M-tiles needs
 extern "C" long lah_ragged_tiles_room(long R, int E) { return R / BM + E + 2; }
 
@@ -1388,37 +1487,84 @@ extern "C" void lah_ragged_nn(const void* d, const void* w, void* out, const voi
 // part in the mean. 2 experts of 131072 rows, 512 x 512 (8 tiles): 2655 us in one part, 146 in
 // 32, 221 in 64; 8 with 13123 of 32768 rows, 1024 x 1024 (128 tiles), 272 in one, 160 in 2, 117
 // in 4, 171 in 8; 16 of 1024 rows, 512 x 512, 31 in one and 37 in 4.
-extern "C" int lah_ragged_splits(long R, int E, int N, int M) {
+static int splits_of(long R, int E, int N, int M) {
   const long tiles = weight_tiles(E, N, M), most = R / E / 256;
   const long s = tiles < 64 ? 256 / tiles : tiles < 256 ? 512 / tiles : 1;
   return (int)(s < most ? s : most < 1 ? 1 : most);
 }
 
+// Lists by rows where there are many tiles and rows, pieces of half a CU's share and at
+// least 16 stages. 256 experts with 15358 rows down to none, 262144 in all, 4096 x 1024: 2403 us
+// in the experts' order, 2254 back and forth, 2167 by rows. 145 experts, one with 15082 of 99929
+// rows (7 L), 248 x 2632: 428 us by rows, 287 in pieces of all above L, 319 of all above 2 L;
+// 128, 12745 of 131072 (3.1 L), 1024 x 1024: 386, 400 and 335; 64, 10002 of 262144 (1.2 L): 490,
+// 561 and 490. Few rows are bound by the stores, which the longer tiles' products then no
+// longer hide: 1024 experts, 32768 rows, 1280 down to none, 512 x 2048: 404 us and 450 by rows.
+static WeightWork weight_work(long R, int E, int N, int M) {
+  WeightWork w{splits_of(R, E, N, M), 0, 0, 0, 0};
+  const long one = (long)M * (N + 1) * 4, tiles = weight_tiles(1, N, M);
+  if (w.splits > 1) {
+    w.bytes = w.splits * E * one;
+  } else if (E > 1 && E <= ORDERED && R / 256 >= E && tiles * E > 256) {
+    const long half = R * tiles / 256 / 2;
+    w.L = ((half > 1024 ? half : 1024) + 63) & ~63l;
+    w.room = (int)(2 * R / w.L) + 1;
+    w.sums = ((2l * w.room + E + 2) * 16 + E * 4 + 255) & ~255l;
+    w.bytes = w.sums + w.room * one;
+  }
+  return w;
+}
+
+extern "C" long lah_ragged_tn_work(long R, int E, int N, int M) { return weight_work(R, E, N, M).bytes; }
+
 // dw[e] = sum_r d[r] x[r]^T: d [R, M], x [R, N], dw [E, M, N]; db [E, M] or null;
-// work: for several splits fp32 room for splits * E * M * (N + 1), else room for an order or null
+// work: lah_ragged_tn_work bytes
 extern "C" void lah_ragged_tn(const void* d, const void* x, void* dw, void* db, int db_bf16,
-                              const void* offsets, long R, int E, int N, int M, int out, int splits,
-                              void* work, hipStream_t stream) {
+                              const void* offsets, long R, int E, int N, int M, int out, void* work,
+                              hipStream_t stream) {
+  const WeightWork need = weight_work(R, E, N, M);
   RaggedArgs a{(const __bf16*)x, (const __bf16*)d, dw, (const int*)offsets, nullptr, nullptr,
-               db, R, E, N, M, 0, db_bf16, splits, false};
-  if (splits > 1) {
-    const long n = (long)E * M * N;
-    float* db_part = (float*)work + splits * n;
+               db, R, E, N, M, 0, db_bf16, need.splits, false};
+  const long n = (long)M * N;
+  if (need.splits > 1) {
+    const int splits = need.splits;
+    float* db_part = (float*)work + splits * E * n;
     a.C = work;
     a.db = db != nullptr ? db_part : nullptr;
     a.bias_bf16 = 0;
     launch_weights<R_F32>(a, nullptr, stream);
-    join((const float*)work, splits, n, dw, out, stream);
+    join((const float*)work, splits, E * n, dw, out, stream);
     if (db != nullptr)
       join(db_part, splits, (long)E * M, db, db_bf16 ? R_BF16 : out == R_F32_ACC ? R_F32_ACC : R_F32, stream);
     return;
   }
-  int* const order = (int*)work;
-  if (order != nullptr)
+  const int4* table = nullptr;
+  if (need.L > 0) {
+    int4* const pieces = (int4*)work;
+    int4* const joins = pieces + need.room + 1;
+    int4* const whole = joins + need.room;
+    int* const order = (int*)(whole + E + 1);
+    float* const part = (float*)((char*)work + need.sums);
     hipLaunchKernelGGL(ragged_order_kernel, dim3(cdiv(E, 256)), dim3(256), 0, stream, a.offsets, E, R, order);
-  if (out == R_BF16) launch_weights<R_BF16>(a, order, stream);
-  else if (out == R_F32_ACC) launch_weights<R_F32_ACC>(a, order, stream);
-  else launch_weights<R_F32>(a, order, stream);
+    hipLaunchKernelGGL(ragged_pieces_kernel, dim3(1), dim3(1024), 0, stream, a.offsets, E, R, need.L, need.room,
+                       (const int*)order, pieces, joins, whole);
+    const dim3 grid((unsigned)((n + M + 1023) / 1024), (unsigned)(R / need.L < E ? R / need.L : E));
+    if (grid.y > 0) {  // some may have more than L rows
+      RaggedArgs p = a;
+      p.C = part;
+      p.db = db != nullptr ? part + need.room * n : nullptr;
+      p.bias_bf16 = 0;
+      launch_weights<R_F32>(p, pieces, stream);
+      auto join_pieces = out == R_BF16 ? ragged_join_pieces_kernel<R_BF16>
+                         : out == R_F32_ACC ? ragged_join_pieces_kernel<R_F32_ACC> : ragged_join_pieces_kernel<R_F32>;
+      hipLaunchKernelGGL(join_pieces, grid, dim3(256), 0, stream, a, (const int4*)pieces, (const int4*)joins,
+                         need.room, (const float*)part);
+    }
+    table = whole;
+  }
+  if (out == R_BF16) launch_weights<R_BF16>(a, table, stream);
+  else if (out == R_F32_ACC) launch_weights<R_F32_ACC>(a, table, stream);
+  else launch_weights<R_F32>(a, table, stream);
 }
 
 // dP = dy * slope, rounded to bf16 for the two products that take it

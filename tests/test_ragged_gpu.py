@@ -373,6 +373,31 @@ class TestGroupedLinear:
         for name in got:
             close(name, got[name], want[name], tol[name])
 
+    @pytest.mark.parametrize("gelu", [False, True])
+    def test_weight_gradients_in_pieces(self, gelu):
+        """Some experts with many more rows than others, more tiles than blocks: pieces for them."""
+        counts = [0, 30000, 1, 500, 6400, 0, 64, 12345] + [300] * 42
+        p = problem(counts, 776, 264, tail=9, bias=torch.bfloat16 if gelu else torch.float32)
+        want, tol = exact(*p, gelu)
+        got = run_all(*p, gelu)
+        for name in got:
+            close(name, got[name], want[name], tol[name])
+        again = run_all(*p, gelu)
+        for name in got:
+            assert torch.equal(got[name], again[name])
+        x, dy = p[0], p[4]
+        for accumulate in (False, True):  # a stack's own sums
+            from learning_at_home_amd.ops import _C
+
+            dw = torch.ones(len(counts), 264, 776, device=DEV)
+            db = torch.ones(len(counts), 264, device=DEV)
+            _C.ragged_tn(dy, x, p[3], dw, db, accumulate)
+            want, tol = exact(x, p[1], None, p[3], dy, False)
+            # without the rounding to bf16; the sum with what was there is rounded once more
+            for name, g in (("dw", dw), ("db", db)):
+                close(name, g, want[name] + accumulate,
+                      tol[name] - BF * want[name].abs() + 2.0 ** -23 * (want[name].abs() + 1))
+
     def test_weights_past_the_cache(self):
         p = problem([3] * 38 + [0, 140], 2056, 2048, tail=3)
         assert p[1].numel() * 2 > 256 << 20
