@@ -99,7 +99,6 @@ LAH_DEVINL void wait_loads_and_barrier() {
 }
 
 LAH_DEVINL void wait_reads_and_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-LAH_DEVINL void barrier() { asm volatile("s_barrier" ::: "memory"); }
 
 // LDS places of 16-byte chunks, so that the 16 lanes that are served together hit
 // 16 different places mod 256 bytes (64 banks).
@@ -1508,7 +1507,7 @@ static WeightWork weight_work(long R, int E, int N, int M) {
   } else if (E > 1 && E <= ORDERED && R / 256 >= E && tiles * E > 256) {
     const long half = R * tiles / 256 / 2;
     w.L = ((half > 1024 ? half : 1024) + 63) & ~63l;
-    w.room = (int)(2 * R / w.L) + 1;
+    w.room = R > w.L ? (int)(2 * R / w.L) + 1 : 0;
     w.sums = ((2l * w.room + E + 2) * 16 + E * 4 + 255) & ~255l;
     w.bytes = w.sums + w.room * one;
   }

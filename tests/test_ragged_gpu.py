@@ -373,6 +373,14 @@ class TestGroupedLinear:
         for name in got:
             close(name, got[name], want[name], tol[name])
 
+    def test_weight_gradients_of_wide_outputs(self):
+        """More than 256 tiles an expert: none is worth pieces."""
+        p = problem([600, 0, 400], 4352, 4360)
+        want, tol = exact(*p, False)
+        got = run_all(*p, False)
+        for name in got:
+            close(name, got[name], want[name], tol[name])
+
     @pytest.mark.parametrize("gelu", [False, True])
     def test_weight_gradients_in_pieces(self, gelu):
         """Some experts with many more rows than others, more tiles than blocks: pieces for them."""
