@@ -70,6 +70,14 @@ hipStream_t cur_stream() { return at::hip::getCurrentHIPStream().stream(); }
 #define CHECK_I32(t) TORCH_CHECK((t).scalar_type() == at::kInt, #t " must be int32")
 #define CHECK_CONTIG(t) TORCH_CHECK((t).is_contiguous(), #t " must be contiguous")
 #define CHECK_CUDA(t) TORCH_CHECK((t).is_cuda(), #t " must be on GPU")
+// Work goes to the tensors' own device, on its current stream.
+#define ON_DEVICE_OF(t) const c10::OptionalDeviceGuard device_guard(at::device_of(t))
+
+// contiguous, from a multiple of 16 bytes on: what the kernels load
+torch::Tensor ready(const torch::Tensor& t) {
+  const auto c = t.contiguous();
+  return ((uintptr_t)c.data_ptr() & 15) == 0 ? c : c.clone();
+}
 
 // C[e] = A[e] @ B[e]^T with fused epilogue; see ffn_gemm.hip
 torch::Tensor batched_gemm_nt(torch::Tensor A, torch::Tensor B,
@@ -205,10 +213,31 @@ std::vector<torch::Tensor> assign_slots(torch::Tensor topk_idx, int64_t E, int64
   return {pos, counts, inv};
 }
 
+// What a kernel of dispatch.hip takes rows and slots from: [T, k] int32, on the rows' GPU
+static void check_slots(const torch::Tensor& rows, const torch::Tensor& topk_idx, const torch::Tensor& pos) {
+  CHECK_CUDA(rows);
+  CHECK_I32(topk_idx); CHECK_I32(pos);
+  TORCH_CHECK(topk_idx.dim() == 2 && topk_idx.sizes() == pos.sizes(), "topk_idx and pos must be [T, k]");
+  TORCH_CHECK(topk_idx.device() == rows.device() && pos.device() == rows.device(),
+              "all tensors must be on one GPU");
+}
+
+static void check_buffer(const torch::Tensor& buf) {
+  CHECK_BF16(buf);
+  TORCH_CHECK(buf.dim() == 3, "the buffer must be [E, C, D]");
+  TORCH_CHECK(buf.size(2) % 8 == 0, "D must be a multiple of 8");
+}
+
 torch::Tensor dispatch_gather(torch::Tensor x, torch::Tensor inv, int64_t k) {
-  CHECK_BF16(x); CHECK_CONTIG(x); CHECK_I32(inv); CHECK_CONTIG(inv);
+  CHECK_CUDA(x); CHECK_BF16(x); CHECK_I32(inv);
+  TORCH_CHECK(x.dim() == 2 && inv.dim() == 2 && x.device() == inv.device(),
+              "x must be [T, D] and inv [E, C], on one GPU");
   int E = inv.size(0), C = inv.size(1), D = x.size(1);
   TORCH_CHECK(D % 8 == 0, "D must be a multiple of 8");
+  TORCH_CHECK(k > 0 || inv.numel() == 0, "k must be positive");
+  ON_DEVICE_OF(x);
+  x = ready(x);
+  inv = inv.contiguous();
   auto xbuf = torch::empty({E, C, D}, x.options());
   lah_dispatch_gather(x.data_ptr(), inv.data_ptr(), xbuf.data_ptr(), E, C, D, (int)k,
                       cur_stream());
@@ -217,8 +246,14 @@ torch::Tensor dispatch_gather(torch::Tensor x, torch::Tensor inv, int64_t k) {
 
 torch::Tensor dispatch_bwd(torch::Tensor dxbuf, torch::Tensor topk_idx, torch::Tensor pos,
                            int64_t T) {
-  CHECK_BF16(dxbuf); CHECK_CONTIG(dxbuf);
+  check_buffer(dxbuf);
+  check_slots(dxbuf, topk_idx, pos);
+  TORCH_CHECK(topk_idx.size(0) == T, "topk_idx must be [T, k]");
   int C = dxbuf.size(1), D = dxbuf.size(2), k = topk_idx.size(1);
+  ON_DEVICE_OF(dxbuf);
+  dxbuf = ready(dxbuf);
+  topk_idx = topk_idx.contiguous();
+  pos = pos.contiguous();
   auto dx = torch::empty({T, D}, dxbuf.options());
   lah_dispatch_bwd(dxbuf.data_ptr(), topk_idx.data_ptr(), pos.data_ptr(), dx.data_ptr(),
                    (int)T, D, k, C, cur_stream());
@@ -227,9 +262,17 @@ torch::Tensor dispatch_bwd(torch::Tensor dxbuf, torch::Tensor topk_idx, torch::T
 
 torch::Tensor combine_fwd(torch::Tensor ybuf, torch::Tensor topk_idx, torch::Tensor pos,
                           torch::Tensor w) {
-  CHECK_BF16(ybuf); CHECK_CONTIG(ybuf); CHECK_F32(w);
+  check_buffer(ybuf);
+  check_slots(ybuf, topk_idx, pos);
+  CHECK_F32(w);
+  TORCH_CHECK(w.sizes() == pos.sizes() && w.device() == ybuf.device(), "w must be [T, k] on the GPU of ybuf");
   int C = ybuf.size(1), D = ybuf.size(2);
   int T = topk_idx.size(0), k = topk_idx.size(1);
+  ON_DEVICE_OF(ybuf);
+  ybuf = ready(ybuf);
+  topk_idx = topk_idx.contiguous();
+  pos = pos.contiguous();
+  w = w.contiguous();
   auto y = torch::empty({T, D}, ybuf.options());
   lah_combine_fwd(ybuf.data_ptr(), topk_idx.data_ptr(), pos.data_ptr(), w.data_ptr(),
                   y.data_ptr(), T, D, k, C, cur_stream());
@@ -240,14 +283,30 @@ std::vector<torch::Tensor> combine_bwd(torch::Tensor dy, torch::Tensor ybuf,
                                        torch::Tensor y, torch::Tensor topk_idx,
                                        torch::Tensor pos, torch::Tensor w,
                                        torch::Tensor inv) {
-  CHECK_BF16(dy); CHECK_BF16(ybuf); CHECK_BF16(y);
+  CHECK_BF16(dy); CHECK_BF16(y); CHECK_F32(w); CHECK_I32(inv);
+  check_buffer(ybuf);
+  check_slots(ybuf, topk_idx, pos);
   int E = ybuf.size(0), C = ybuf.size(1), D = ybuf.size(2);
   int T = topk_idx.size(0), k = topk_idx.size(1);
+  TORCH_CHECK(w.sizes() == pos.sizes() && inv.dim() == 2 && inv.size(0) == E && inv.size(1) == C,
+              "w must be [T, k] and inv [E, C]");
+  TORCH_CHECK(y.dim() == 2 && y.size(0) == T && y.size(1) == D && dy.sizes() == y.sizes(),
+              "dy and y must be [T, D]");
+  for (const auto* t : {&dy, &y, &w, &inv})
+    TORCH_CHECK(t->device() == ybuf.device(), "all tensors must be on one GPU");
+  ON_DEVICE_OF(ybuf);
+  dy = ready(dy);
+  ybuf = ready(ybuf);
+  y = ready(y);
+  topk_idx = topk_idx.contiguous();
+  pos = pos.contiguous();
+  w = w.contiguous();
+  inv = inv.contiguous();
   auto dybuf = torch::empty({E, C, D}, ybuf.options());
   auto dw = torch::empty({T, k}, w.options());
   // padding rows (inv < 0) are zero-filled; surviving rows written by scatter
   lah_zero_padding(inv.data_ptr(), dybuf.data_ptr(), E, C, D, cur_stream());
-  lah_combine_bwd(dy.contiguous().data_ptr(), ybuf.data_ptr(), y.data_ptr(),
+  lah_combine_bwd(dy.data_ptr(), ybuf.data_ptr(), y.data_ptr(),
                   topk_idx.data_ptr(), pos.data_ptr(), w.data_ptr(), dybuf.data_ptr(),
                   dw.data_ptr(), T, D, k, C, cur_stream());
   return {dybuf, dw};
@@ -376,8 +435,6 @@ std::vector<torch::Tensor> flash_attn_bwd(torch::Tensor q, torch::Tensor k,
 
 // ---- products grouped by expert, ragged sizes (ragged_gemm.hip, ragged_layout.hip) ----
 
-// Work goes to the tensors' own device, on its current stream.
-#define ON_DEVICE_OF(t) const c10::OptionalDeviceGuard device_guard(at::device_of(t))
 #define CHECK_LAUNCH()                                                      \
   do {                                                                      \
     const hipError_t err = hipGetLastError();                               \
@@ -568,12 +625,6 @@ torch::Tensor ragged_slope(torch::Tensor dy, torch::Tensor der) {
 }
 
 // ---- the differentiable product ----
-
-// contiguous, from a multiple of 16 bytes on: what the kernels load
-static torch::Tensor ready(const torch::Tensor& t) {
-  const auto c = t.contiguous();
-  return ((uintptr_t)c.data_ptr() & 15) == 0 ? c : c.clone();
-}
 
 struct GroupedLinear : public torch::autograd::Function<GroupedLinear> {
   static torch::Tensor forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& x_in,

@@ -63,27 +63,68 @@ def ragged_layout(topk_idx: torch.Tensor, num_experts: int) -> RaggedLayout:
                         torch.where(key < num_experts, rows, -1).int().view(topk_idx.shape))
 
 
+def _check_layout(layout, t, name):
+    """The layout's parts go together, and with t: the kernels take rows and slots from them."""
+    rows, order = layout.rows, layout.order
+    if rows.dtype != torch.int32 or order.dtype != torch.int32:
+        raise ValueError(f"the layout's order and rows must be int32, got {order.dtype} and {rows.dtype}")
+    if rows.dim() != 2 or order.shape != (rows.numel(),):
+        raise ValueError(f"the layout must have rows [T, k] and order [T * k], got {tuple(rows.shape)} "
+                         f"and {tuple(order.shape)}")
+    if not t.device == rows.device == order.device:
+        raise ValueError(f"{name} and the layout must be on one device")
+
+
+def _check_gpu_rows(t, name):
+    if t.dtype != torch.bfloat16:
+        raise ValueError(f"the GPU kernels take bf16, got {name} in {t.dtype}")
+    if t.shape[1] % 8:
+        raise ValueError(f"{name} must have a multiple of 8 columns (16-byte rows), got {tuple(t.shape)}")
+
+
 def ragged_gather(x: torch.Tensor, layout: RaggedLayout) -> torch.Tensor:
-    """x [T, D] -> the layout's rows [T * k, D]; rows of nobody are zeros."""
+    """x [T, D] -> the layout's rows [T * k, D]; rows of nobody are zeros. On a
+    GPU: bf16, D a multiple of 8."""
     from .functional import dispatch
 
+    _check_layout(layout, x, "x")
+    T, k = layout.rows.shape
+    if x.dim() != 2 or x.shape[0] != T:
+        raise ValueError(f"x must be [{T}, D], a row for each token of the layout, got {tuple(x.shape)}")
+    if x.is_cuda and HAS_HIP:
+        _check_gpu_rows(x, "x")
+        x = _ready(x)
     one = torch.zeros_like(layout.rows)  # all rows in one group: their number is their slot
-    return dispatch(x, one, layout.rows, layout.order.unsqueeze(0), layout.rows.shape[1])[0]
+    return dispatch(x, one, layout.rows, layout.order.unsqueeze(0), k)[0]
 
 
 def ragged_ungather(y: torch.Tensor, layout: RaggedLayout) -> torch.Tensor:
     """y [T * k, D] -> [T * k, D], row of slot t * k + j at its place again (each
-    slot's own row, not summed); zeros for slots that have none."""
-    weights = torch.ones(layout.rows.numel(), 1, device=y.device)
+    slot's own row, not summed); zeros for slots that have none. On a GPU: bf16, D
+    a multiple of 8."""
+    weights = torch.ones(layout.rows.numel(), 1, device=y.device, dtype=torch.float32)
     rows = layout.rows.reshape(-1, 1)
     return ragged_combine(y, RaggedLayout(layout.offsets, layout.order, rows), weights)
 
 
 def ragged_combine(y: torch.Tensor, layout: RaggedLayout, weights: torch.Tensor) -> torch.Tensor:
     """y [T * k, D] -> [T, D], each token's rows by its weights [T, k], which are
-    normalised over the slots that have a row (functional.combine)."""
+    normalised over the slots that have a row (functional.combine). On a GPU: y
+    bf16, D a multiple of 8, weights fp32."""
     from .functional import combine
 
+    _check_layout(layout, y, "y")
+    if y.dim() != 2 or y.shape[0] != layout.order.numel():
+        raise ValueError(f"y must be [{layout.order.numel()}, D], the layout's rows, got {tuple(y.shape)}")
+    if weights.shape != layout.rows.shape:
+        raise ValueError(f"weights must be {tuple(layout.rows.shape)}, one for each slot, got {tuple(weights.shape)}")
+    if weights.device != y.device:
+        raise ValueError("y, weights and the layout must be on one device")
+    if y.is_cuda and HAS_HIP:
+        _check_gpu_rows(y, "y")
+        if weights.dtype != torch.float32:
+            raise ValueError(f"weights must be fp32, got {weights.dtype}")
+        y = _ready(y)
     one = torch.zeros_like(layout.rows)
     return combine(y.unsqueeze(0), one, layout.rows, weights, layout.order.unsqueeze(0))
 
