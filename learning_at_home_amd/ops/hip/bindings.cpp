@@ -72,6 +72,11 @@ hipStream_t cur_stream() { return at::hip::getCurrentHIPStream().stream(); }
 #define CHECK_CUDA(t) TORCH_CHECK((t).is_cuda(), #t " must be on GPU")
 // Work goes to the tensors' own device, on its current stream.
 #define ON_DEVICE_OF(t) const c10::OptionalDeviceGuard device_guard(at::device_of(t))
+#define CHECK_LAUNCH()                                                      \
+  do {                                                                      \
+    const hipError_t err = hipGetLastError();                               \
+    TORCH_CHECK(err == hipSuccess, "launch: ", hipGetErrorString(err));     \
+  } while (0)
 
 // contiguous, from a multiple of 16 bytes on: what the kernels load
 torch::Tensor ready(const torch::Tensor& t) {
@@ -179,11 +184,13 @@ std::vector<torch::Tensor> gating_topk_fwd(torch::Tensor logits, int64_t k) {
   TORCH_CHECK(E <= 4096, "gating kernel supports up to 4096 experts, got ", E);
   TORCH_CHECK(k == 1 || k == 2 || k == 4 || k == 8,
               "gating kernel supports k in {1,2,4,8}, got ", k);
+  ON_DEVICE_OF(logits);
   auto probs = torch::empty({T, E}, logits.options().dtype(at::kBFloat16));
   auto topk_idx = torch::empty({T, k}, logits.options().dtype(at::kInt));
   auto topk_w = torch::empty({T, k}, logits.options());
   lah_gating_topk_fwd(logits.data_ptr(), probs.data_ptr(), topk_idx.data_ptr(),
                       topk_w.data_ptr(), T, E, (int)k, cur_stream());
+  CHECK_LAUNCH();
   return {probs, topk_idx, topk_w};
 }
 
@@ -199,6 +206,7 @@ torch::Tensor gating_topk_bwd(torch::Tensor probs, torch::Tensor topk_idx,
   lah_gating_topk_bwd(probs.data_ptr(), topk_idx.data_ptr(), topk_w.data_ptr(),
                       d_topk_w.contiguous().data_ptr(), aux_p, d_logits.data_ptr(), T, E, k,
                       cur_stream());
+  CHECK_LAUNCH();
   return d_logits;
 }
 
@@ -210,6 +218,7 @@ std::vector<torch::Tensor> assign_slots(torch::Tensor topk_idx, int64_t E, int64
   auto inv = torch::full({E, C}, -1, topk_idx.options());
   lah_assign_slots(topk_idx.data_ptr(), pos.data_ptr(), counts.data_ptr(), inv.data_ptr(),
                    T, k, (int)C, (int)E, cur_stream());
+  CHECK_LAUNCH();
   return {pos, counts, inv};
 }
 
@@ -241,6 +250,7 @@ torch::Tensor dispatch_gather(torch::Tensor x, torch::Tensor inv, int64_t k) {
   auto xbuf = torch::empty({E, C, D}, x.options());
   lah_dispatch_gather(x.data_ptr(), inv.data_ptr(), xbuf.data_ptr(), E, C, D, (int)k,
                       cur_stream());
+  CHECK_LAUNCH();
   return xbuf;
 }
 
@@ -257,6 +267,7 @@ torch::Tensor dispatch_bwd(torch::Tensor dxbuf, torch::Tensor topk_idx, torch::T
   auto dx = torch::empty({T, D}, dxbuf.options());
   lah_dispatch_bwd(dxbuf.data_ptr(), topk_idx.data_ptr(), pos.data_ptr(), dx.data_ptr(),
                    (int)T, D, k, C, cur_stream());
+  CHECK_LAUNCH();
   return dx;
 }
 
@@ -276,6 +287,7 @@ torch::Tensor combine_fwd(torch::Tensor ybuf, torch::Tensor topk_idx, torch::Ten
   auto y = torch::empty({T, D}, ybuf.options());
   lah_combine_fwd(ybuf.data_ptr(), topk_idx.data_ptr(), pos.data_ptr(), w.data_ptr(),
                   y.data_ptr(), T, D, k, C, cur_stream());
+  CHECK_LAUNCH();
   return y;
 }
 
@@ -309,6 +321,7 @@ std::vector<torch::Tensor> combine_bwd(torch::Tensor dy, torch::Tensor ybuf,
   lah_combine_bwd(dy.data_ptr(), ybuf.data_ptr(), y.data_ptr(),
                   topk_idx.data_ptr(), pos.data_ptr(), w.data_ptr(), dybuf.data_ptr(),
                   dw.data_ptr(), T, D, k, C, cur_stream());
+  CHECK_LAUNCH();
   return {dybuf, dw};
 }
 
@@ -435,11 +448,6 @@ std::vector<torch::Tensor> flash_attn_bwd(torch::Tensor q, torch::Tensor k,
 
 // ---- products grouped by expert, ragged sizes (ragged_gemm.hip, ragged_layout.hip) ----
 
-#define CHECK_LAUNCH()                                                      \
-  do {                                                                      \
-    const hipError_t err = hipGetLastError();                               \
-    TORCH_CHECK(err == hipSuccess, "launch: ", hipGetErrorString(err));     \
-  } while (0)
 #define CHECK_ALIGNED(t) \
   TORCH_CHECK(((uintptr_t)(t).data_ptr() & 15) == 0, #t " must start at a multiple of 16 bytes")
 

@@ -183,10 +183,13 @@ __global__ void zero_padding_kernel(const int* __restrict__ inv, __bf16* __restr
 }
 
 // ---- launchers -------------------------------------------------------------
+// An empty grid is an error that the next check of another call would report: a batch
+// without tokens, or a rank that gets no rows, launches nothing.
 extern "C" void lah_assign_slots(const void* topk_idx, void* pos, void* counts,
                                  void* inv, int T, int k, int C, int E,
                                  hipStream_t stream) {
   int total = T * k;
+  if (total == 0) return;
   hipLaunchKernelGGL(assign_slots_kernel, dim3(cdiv(total, 256)), dim3(256), 0, stream,
                      (const int*)topk_idx, (int*)pos, (int*)counts, (int*)inv, total, C, E);
 }
@@ -194,12 +197,14 @@ extern "C" void lah_assign_slots(const void* topk_idx, void* pos, void* counts,
 extern "C" void lah_dispatch_gather(const void* x, const void* inv, void* xbuf, int E,
                                     int C, int D, int k, hipStream_t stream) {
   int rows = E * C;
+  if (rows == 0) return;
   hipLaunchKernelGGL(dispatch_gather_kernel, dim3(cdiv(rows, 4)), dim3(256), 0, stream,
                      (const __bf16*)x, (const int*)inv, (__bf16*)xbuf, rows, D, k);
 }
 
 extern "C" void lah_dispatch_bwd(const void* dxbuf, const void* topk_idx, const void* pos,
                                  void* dx, int T, int D, int k, int C, hipStream_t stream) {
+  if (T == 0) return;
   hipLaunchKernelGGL(dispatch_bwd_kernel, dim3(cdiv(T, 4)), dim3(256), 0, stream,
                      (const __bf16*)dxbuf, (const int*)topk_idx, (const int*)pos,
                      (__bf16*)dx, T, D, k, C);
@@ -208,6 +213,7 @@ extern "C" void lah_dispatch_bwd(const void* dxbuf, const void* topk_idx, const 
 extern "C" void lah_combine_fwd(const void* ybuf, const void* topk_idx, const void* pos,
                                 const void* w, void* y, int T, int D, int k, int C,
                                 hipStream_t stream) {
+  if (T == 0) return;
   hipLaunchKernelGGL(combine_fwd_kernel, dim3(cdiv(T, 4)), dim3(256), 0, stream,
                      (const __bf16*)ybuf, (const int*)topk_idx, (const int*)pos,
                      (const float*)w, (__bf16*)y, T, D, k, C);
@@ -217,6 +223,7 @@ extern "C" void lah_combine_bwd(const void* dy, const void* ybuf, const void* y,
                                 const void* topk_idx, const void* pos, const void* w,
                                 void* dybuf, void* dw, int T, int D, int k, int C,
                                 hipStream_t stream) {
+  if (T == 0) return;
   hipLaunchKernelGGL(combine_bwd_kernel, dim3(cdiv(T, 4)), dim3(256), 0, stream,
                      (const __bf16*)dy, (const __bf16*)ybuf, (const __bf16*)y,
                      (const int*)topk_idx, (const int*)pos, (const float*)w,
@@ -226,6 +233,7 @@ extern "C" void lah_combine_bwd(const void* dy, const void* ybuf, const void* y,
 extern "C" void lah_zero_padding(const void* inv, void* buf, int E, int C, int D,
                                  hipStream_t stream) {
   int rows = E * C;
+  if (rows == 0) return;
   hipLaunchKernelGGL(zero_padding_kernel, dim3(cdiv(rows, 4)), dim3(256), 0, stream,
                      (const int*)inv, (__bf16*)buf, rows, D);
 }

@@ -169,6 +169,7 @@ __global__ void gating_topk_bwd_kernel(const __bf16* __restrict__ probs,   // [T
 extern "C" void lah_gating_topk_fwd(const void* logits, void* probs, void* topk_idx,
                                     void* topk_w, int T, int E, int k,
                                     hipStream_t stream) {
+  if (T == 0) return;  // an empty grid is an error
   dim3 grid(cdiv(T, GATE_WAVES)), block(GATE_WAVES * 64);
   int epl = cdiv(E, 64);
 #define CASE_K(N, K)                                                                   \
@@ -192,6 +193,7 @@ extern "C" void lah_gating_topk_bwd(const void* probs, const void* topk_idx,
                                     const void* topk_w, const void* d_topk_w,
                                     const void* aux_g, void* d_logits, int T, int E,
                                     int k, hipStream_t stream) {
+  if (T == 0) return;  // an empty grid is an error
   dim3 grid(cdiv(T, GATE_WAVES)), block(GATE_WAVES * 64);
   int epl = cdiv(E, 64);
 #define CASE(N)                                                                        \

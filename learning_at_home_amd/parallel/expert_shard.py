@@ -702,6 +702,8 @@ class ExpertParallelMoE(nn.Module):
                     T: int) -> Optional[torch.Tensor]:
         E, k = self.num_experts, self.k
         aux = None
+        if T == 0:  # no tokens, no loss of theirs: a mean over none is not a number
+            return logits.sum() if self.aux_loss_coef > 0 or self.z_loss_coef > 0 else None
         if self.aux_loss_coef > 0:
             f = (counts.float() / max(1, T * k)).detach()
             mean_probs = probs.float().mean(dim=0)

@@ -1,10 +1,16 @@
 """Calls at the edges of the ragged expert path, on the CPU: arguments that do not go
 together, no tokens, weights of little mass, derivatives that the operators do not have."""
+import os
+import socket
+
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from learning_at_home_amd.ops import functional as Fops
 from learning_at_home_amd.ops import ragged
+from learning_at_home_amd.parallel import ExpertParallelMoE
 
 
 def layout_of(ids, E):
@@ -56,3 +62,48 @@ class TestRowsRefuse:
     def test_what_the_kernels_do_not_take(self, t, match):
         with pytest.raises(ValueError, match=match):
             ragged._check_gpu_rows(t, "x")
+
+
+@pytest.mark.parametrize("dropless", [False, True])
+def test_layer_without_tokens(dropless):
+    """A rank whose batch is empty: no rows, no gradients, losses of zero."""
+    moe = ExpertParallelMoE(16, 32, 8, k=2, dropless=dropless, z_loss_coef=0.1)
+    x = torch.randn(0, 16, requires_grad=True)
+    y = moe(x)
+    assert y.shape == (0, 16) and moe.aux_loss == 0 and not moe.last_counts.any()
+    (y.sum() + moe.aux_loss).backward()
+    assert x.grad.shape == (0, 16) and not moe.gate.weight.grad.any()
+
+
+def _idle_worker(rank, port, x, queue):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    torch.manual_seed(0)
+    moe = ExpertParallelMoE(16, 32, 8, k=2, dropless=True, router_noise_std=0.0)
+    with torch.no_grad():
+        moe.gate.weight.copy_(torch.arange(8, 0, -1)[:, None].expand(8, 16))  # experts 0 and 1, rank 0's
+    leaf = (x if rank == 0 else x[:0]).clone().requires_grad_(True)
+    y = moe(leaf)
+    (y.sum() + moe.aux_loss).backward()
+    queue.put((rank, y.shape[0], leaf.grad.shape[0], int(moe.last_counts.sum()),
+               bool(moe.experts.W1.grad.any()) if moe.experts.W1.grad is not None else None))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_idle_rank_over_gloo():
+    """One rank has no tokens and is sent none: it takes part in every exchange all the same."""
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    x = torch.rand(7, 16) + 0.1
+    ctx = mp.get_context("spawn")
+    queue = ctx.Queue()
+    procs = [ctx.Process(target=_idle_worker, args=(r, port, x, queue)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict((r[0], r[1:]) for r in (queue.get(timeout=120) for _ in procs))
+    for p in procs:
+        p.join(60)
+    assert got[0] == (7, 7, 14, True)
+    assert got[1][:3] == (0, 0, 0) and not got[1][3]

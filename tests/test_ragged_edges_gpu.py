@@ -7,6 +7,7 @@ pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
     from learning_at_home_amd.ops import functional as Fops
+    from learning_at_home_amd.parallel import ExpertParallelMoE, ExpertStack
 
 DEV = "cuda:0"
 BF = 2.0 ** -8  # one rounding to bf16: half a step
@@ -70,3 +71,55 @@ def test_rows_from_views():
     for got in (run(off(x), off(w), off(dy)), run(wide[:, 5:29], pairs[:, ::2], off(dy))):
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+class TestNoTokens:
+    def make_stack(self):
+        torch.manual_seed(0)
+        stack = ExpertStack(4, 128, 256).to(DEV)
+        stack.init_gpu_state()
+        return stack
+
+    def test_rows(self):
+        """Gather, FFN and combine of no rows, forward and backward; nothing is left for a later check."""
+        stack = self.make_stack()
+        layout = Fops.ragged_layout(torch.empty(0, 2, dtype=torch.int32, device=DEV), 4)
+        x = torch.empty(0, 128, device=DEV).bfloat16().requires_grad_(True)
+        w = torch.empty(0, 2, device=DEV, requires_grad=True)
+        for g in (stack.main_grad_W1, stack.main_grad_W2, stack.main_grad_b1, stack.main_grad_b2):
+            g.fill_(1.0)
+        rows = Fops.ragged_gather(x, layout)
+        out = Fops.ragged_combine(Fops.ragged_ffn(rows, layout.offsets, stack), layout, w)
+        assert rows.shape == out.shape == (0, 128) and Fops.ragged_ungather(rows, layout).shape == (0, 128)
+        out.sum().backward()
+        assert x.grad.shape == (0, 128) and w.grad.shape == (0, 2)
+        for g in (stack.main_grad_W1, stack.main_grad_W2, stack.main_grad_b1, stack.main_grad_b2):
+            assert not g.any()
+        Fops.ragged_layout(torch.zeros(5, 2, dtype=torch.int32, device=DEV), 4)
+        torch.cuda.synchronize()
+
+    def test_rank_without_rows(self):
+        """What a rank does that receives nothing while its own tokens go elsewhere: its layout has
+        experts and no rows, and what it sent comes back."""
+        stack = self.make_stack()
+        arrived = torch.empty(0, 128, device=DEV).bfloat16().requires_grad_(True)
+        layout = Fops.ragged_layout(torch.empty(0, dtype=torch.int32, device=DEV).unsqueeze(1), 4)
+        y = Fops.ragged_ffn(Fops.ragged_gather(arrived, layout), layout.offsets, stack)
+        y = Fops.ragged_ungather(y, layout)
+        y.backward(torch.empty(0, 128, device=DEV).bfloat16())
+        assert arrived.grad.shape == (0, 128) and stack.grad_ready and not stack.main_grad_W1.any()
+        assert not Fops.ragged_layout(torch.full((3, 1), -1, dtype=torch.int32, device=DEV), 4).offsets.any()
+
+    @pytest.mark.parametrize("dropless", [False, True])
+    def test_layer(self, dropless):
+        torch.manual_seed(5)
+        moe = ExpertParallelMoE(128, 256, 8, k=2, dropless=dropless, z_loss_coef=0.1).to(DEV).bfloat16()
+        moe.experts.float()
+        moe.experts.init_gpu_state()
+        x = torch.randn(0, 128, device=DEV).bfloat16().requires_grad_(True)
+        y = moe(x)
+        assert y.shape == (0, 128) and moe.aux_loss == 0 and not moe.last_counts.any()
+        (y.sum() + moe.aux_loss).backward()
+        assert x.grad.shape == (0, 128) and not moe.gate.weight.grad.any()
+        moe(torch.randn(3, 128, device=DEV).bfloat16())  # no error was left behind
+        torch.cuda.synchronize()
