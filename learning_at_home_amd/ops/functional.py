@@ -138,11 +138,12 @@ def dispatch(x, topk_idx, pos, inv, k):
 # ---------------------------------------------------------------------------
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ybuf: torch.Tensor, topk_idx, pos, w, inv):
+    def forward(ctx, ybuf: torch.Tensor, topk_idx, pos, w, inv, min_mass):
         if ybuf.is_cuda and HAS_HIP:
-            y = _C.combine_fwd(ybuf.contiguous(), topk_idx, pos, w.contiguous())
+            y = _C.combine_fwd(ybuf.contiguous(), topk_idx, pos, w.contiguous(), min_mass)
         else:
-            y = _combine_fwd_torch(ybuf, topk_idx, pos, w)
+            y = _combine_fwd_torch(ybuf, topk_idx, pos, w, min_mass)
+        ctx.min_mass = min_mass
         ctx.save_for_backward(ybuf, y, topk_idx, pos, w, inv)
         return y
 
@@ -151,34 +152,34 @@ class _Combine(torch.autograd.Function):
         ybuf, y, topk_idx, pos, w, inv = ctx.saved_tensors
         if dy.is_cuda and HAS_HIP:
             dybuf, dw = _C.combine_bwd(dy.contiguous(), ybuf, y, topk_idx, pos,
-                                       w.contiguous(), inv)
-            return dybuf, None, None, dw, None
-        dybuf, dw = _combine_bwd_torch(dy, ybuf, y, topk_idx, pos, w)
-        return dybuf, None, None, dw, None
+                                       w.contiguous(), inv, ctx.min_mass)
+            return dybuf, None, None, dw, None, None
+        dybuf, dw = _combine_bwd_torch(dy, ybuf, y, topk_idx, pos, w, ctx.min_mass)
+        return dybuf, None, None, dw, None, None
 
 
-def _survivor_weights(pos, w):
+def _survivor_weights(pos, w, min_mass=0.2):
     surv = pos >= 0
     s = (w * surv).sum(-1, keepdim=True)
     # clamped renormalization (matches dispatch.hip): bounds the gradient
     # amplification when capacity drops remove most of the softmax mass
-    inv_s = torch.where(s > 0, 1.0 / s.clamp(min=0.2), torch.zeros_like(s))
+    inv_s = torch.where(s > 0, 1.0 / s.clamp(min=min_mass), torch.zeros_like(s))
     return (w * surv) * inv_s, surv, inv_s
 
 
-def _combine_fwd_torch(ybuf, topk_idx, pos, w):
+def _combine_fwd_torch(ybuf, topk_idx, pos, w, min_mass=0.2):
     E, C, D = ybuf.shape
     T, k = topk_idx.shape
-    w_hat, surv, _ = _survivor_weights(pos, w)
+    w_hat, surv, _ = _survivor_weights(pos, w, min_mass)
     flat = (topk_idx.long() * C + pos.clamp(min=0).long()).view(-1)
     rows = ybuf.view(-1, D)[flat].view(T, k, D)
     return (w_hat.unsqueeze(-1).to(rows.dtype) * rows * surv.unsqueeze(-1)).sum(1)
 
 
-def _combine_bwd_torch(dy, ybuf, y, topk_idx, pos, w):
+def _combine_bwd_torch(dy, ybuf, y, topk_idx, pos, w, min_mass=0.2):
     E, C, D = ybuf.shape
     T, k = topk_idx.shape
-    w_hat, surv, inv_s = _survivor_weights(pos, w)
+    w_hat, surv, inv_s = _survivor_weights(pos, w, min_mass)
     dybuf = torch.zeros_like(ybuf)
     flat_valid = pos.view(-1) >= 0
     flat_slot = (topk_idx.long() * C + pos.clamp(min=0).long()).view(-1)[flat_valid]
@@ -189,13 +190,13 @@ def _combine_bwd_torch(dy, ybuf, y, topk_idx, pos, w):
     dot_yj = torch.einsum("td,tkd->tk", dy.float(), rows.float())
     dot_y = torch.einsum("td,td->t", dy.float(), y.float()).unsqueeze(-1)
     s = (w * surv).sum(-1, keepdim=True)
-    clamped = (s > 0) & (s < 0.2)  # in the clamp region d(w/0.2)/dw is diagonal
+    clamped = (s > 0) & (s < min_mass)  # in the clamp region d(w/min_mass)/dw is diagonal
     dw = (torch.where(clamped, dot_yj, dot_yj - dot_y) * inv_s) * surv
     return dybuf, dw.float()
 
 
-def combine(ybuf, topk_idx, pos, w, inv):
-    return _Combine.apply(ybuf, topk_idx, pos, w, inv)
+def combine(ybuf, topk_idx, pos, w, inv, min_mass=0.2):
+    return _Combine.apply(ybuf, topk_idx, pos, w, inv, min_mass)
 
 
 # ---------------------------------------------------------------------------

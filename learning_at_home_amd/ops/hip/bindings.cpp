@@ -25,9 +25,9 @@ void lah_dispatch_gather(const void*, const void*, void*, int, int, int, int, hi
 void lah_dispatch_bwd(const void*, const void*, const void*, void*, int, int, int, int,
                       hipStream_t);
 void lah_combine_fwd(const void*, const void*, const void*, const void*, void*, int, int,
-                     int, int, hipStream_t);
+                     int, int, float, hipStream_t);
 void lah_combine_bwd(const void*, const void*, const void*, const void*, const void*,
-                     const void*, void*, void*, int, int, int, int, hipStream_t);
+                     const void*, void*, void*, int, int, int, int, float, hipStream_t);
 void lah_zero_padding(const void*, void*, int, int, int, hipStream_t);
 void lah_sgd_step(void*, const void*, void*, void*, long, float, float, float,
                   const void*, hipStream_t);
@@ -272,7 +272,7 @@ torch::Tensor dispatch_bwd(torch::Tensor dxbuf, torch::Tensor topk_idx, torch::T
 }
 
 torch::Tensor combine_fwd(torch::Tensor ybuf, torch::Tensor topk_idx, torch::Tensor pos,
-                          torch::Tensor w) {
+                          torch::Tensor w, double least) {
   check_buffer(ybuf);
   check_slots(ybuf, topk_idx, pos);
   CHECK_F32(w);
@@ -286,7 +286,7 @@ torch::Tensor combine_fwd(torch::Tensor ybuf, torch::Tensor topk_idx, torch::Ten
   w = w.contiguous();
   auto y = torch::empty({T, D}, ybuf.options());
   lah_combine_fwd(ybuf.data_ptr(), topk_idx.data_ptr(), pos.data_ptr(), w.data_ptr(),
-                  y.data_ptr(), T, D, k, C, cur_stream());
+                  y.data_ptr(), T, D, k, C, (float)least, cur_stream());
   CHECK_LAUNCH();
   return y;
 }
@@ -294,7 +294,7 @@ torch::Tensor combine_fwd(torch::Tensor ybuf, torch::Tensor topk_idx, torch::Ten
 std::vector<torch::Tensor> combine_bwd(torch::Tensor dy, torch::Tensor ybuf,
                                        torch::Tensor y, torch::Tensor topk_idx,
                                        torch::Tensor pos, torch::Tensor w,
-                                       torch::Tensor inv) {
+                                       torch::Tensor inv, double least) {
   CHECK_BF16(dy); CHECK_BF16(y); CHECK_F32(w); CHECK_I32(inv);
   check_buffer(ybuf);
   check_slots(ybuf, topk_idx, pos);
@@ -320,7 +320,7 @@ std::vector<torch::Tensor> combine_bwd(torch::Tensor dy, torch::Tensor ybuf,
   lah_zero_padding(inv.data_ptr(), dybuf.data_ptr(), E, C, D, cur_stream());
   lah_combine_bwd(dy.data_ptr(), ybuf.data_ptr(), y.data_ptr(),
                   topk_idx.data_ptr(), pos.data_ptr(), w.data_ptr(), dybuf.data_ptr(),
-                  dw.data_ptr(), T, D, k, C, cur_stream());
+                  dw.data_ptr(), T, D, k, C, (float)least, cur_stream());
   CHECK_LAUNCH();
   return {dybuf, dw};
 }
@@ -816,8 +816,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("assign_slots", &assign_slots);
   m.def("dispatch_gather", &dispatch_gather);
   m.def("dispatch_bwd", &dispatch_bwd);
-  m.def("combine_fwd", &combine_fwd);
-  m.def("combine_bwd", &combine_bwd);
+  m.def("combine_fwd", &combine_fwd, py::arg("ybuf"), py::arg("topk_idx"), py::arg("pos"),
+        py::arg("w"), py::arg("least") = 0.2);
+  m.def("combine_bwd", &combine_bwd, py::arg("dy"), py::arg("ybuf"), py::arg("y"),
+        py::arg("topk_idx"), py::arg("pos"), py::arg("w"), py::arg("inv"), py::arg("least") = 0.2);
   m.def("sgd_step", &sgd_step, py::arg("master"), py::arg("grad"),
         py::arg("momentum"), py::arg("out_bf16"),
         py::arg("lr") = 0.01, py::arg("mu") = 0.0, py::arg("weight_decay") = 0.0,

@@ -82,17 +82,17 @@ __global__ void combine_fwd_kernel(const __bf16* __restrict__ ybuf,   // [E, C, 
                                    const int* __restrict__ pos,       // [T, k]
                                    const float* __restrict__ w,       // [T, k]
                                    __bf16* __restrict__ y,            // [T, D]
-                                   int T, int D, int k, int C) {
+                                   int T, int D, int k, int C, float least) {
   int t = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
   if (t >= T) return;
   int lane = threadIdx.x & 63;
   float s = 0.f;
   for (int j = 0; j < k; ++j)
     if (pos[(long)t * k + j] >= 0) s += w[(long)t * k + j];
-  // clamp the renormalization mass: when capacity drops remove most of the
-  // softmax mass, an unclamped 1/s amplifies combine gradients by up to
-  // 1/w_min and detonates the router (observed at flagship scale)
-  float inv_s = (s > 0.f) ? 1.0f / fmaxf(s, 0.2f) : 0.f;
+  // clamp the renormalization mass (least = 0.2 after capacity drops): when
+  // these remove most of the softmax mass, an unclamped 1/s amplifies combine
+  // gradients by up to 1/w_min and detonates the router (observed at flagship scale)
+  float inv_s = (s > 0.f) ? 1.0f / fmaxf(s, least) : 0.f;
   for (int c = lane * 8; c < D; c += 64 * 8) {
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < k; ++j) {
@@ -122,15 +122,15 @@ __global__ void combine_bwd_kernel(const __bf16* __restrict__ dy,     // [T, D]
                                    const float* __restrict__ w,       // [T, k]
                                    __bf16* __restrict__ dybuf,        // [E, C, D]
                                    float* __restrict__ dw,            // [T, k]
-                                   int T, int D, int k, int C) {
+                                   int T, int D, int k, int C, float least) {
   int t = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
   if (t >= T) return;
   int lane = threadIdx.x & 63;
   float s = 0.f;
   for (int j = 0; j < k; ++j)
     if (pos[(long)t * k + j] >= 0) s += w[(long)t * k + j];
-  float inv_s = (s > 0.f) ? 1.0f / fmaxf(s, 0.2f) : 0.f;  // see combine_fwd
-  bool clamped = (s > 0.f) && (s < 0.2f);  // d(w/0.2)/dw has no quotient term
+  float inv_s = (s > 0.f) ? 1.0f / fmaxf(s, least) : 0.f;  // see combine_fwd
+  bool clamped = (s > 0.f) && (s < least);  // d(w/least)/dw has no quotient term
 
   // <dy, y> once per token
   float dot_dy_y = 0.f;
@@ -212,22 +212,22 @@ extern "C" void lah_dispatch_bwd(const void* dxbuf, const void* topk_idx, const 
 
 extern "C" void lah_combine_fwd(const void* ybuf, const void* topk_idx, const void* pos,
                                 const void* w, void* y, int T, int D, int k, int C,
-                                hipStream_t stream) {
+                                float least, hipStream_t stream) {
   if (T == 0) return;
   hipLaunchKernelGGL(combine_fwd_kernel, dim3(cdiv(T, 4)), dim3(256), 0, stream,
                      (const __bf16*)ybuf, (const int*)topk_idx, (const int*)pos,
-                     (const float*)w, (__bf16*)y, T, D, k, C);
+                     (const float*)w, (__bf16*)y, T, D, k, C, least);
 }
 
 extern "C" void lah_combine_bwd(const void* dy, const void* ybuf, const void* y,
                                 const void* topk_idx, const void* pos, const void* w,
                                 void* dybuf, void* dw, int T, int D, int k, int C,
-                                hipStream_t stream) {
+                                float least, hipStream_t stream) {
   if (T == 0) return;
   hipLaunchKernelGGL(combine_bwd_kernel, dim3(cdiv(T, 4)), dim3(256), 0, stream,
                      (const __bf16*)dy, (const __bf16*)ybuf, (const __bf16*)y,
                      (const int*)topk_idx, (const int*)pos, (const float*)w,
-                     (__bf16*)dybuf, (float*)dw, T, D, k, C);
+                     (__bf16*)dybuf, (float*)dw, T, D, k, C, least);
 }
 
 extern "C" void lah_zero_padding(const void* inv, void* buf, int E, int C, int D,

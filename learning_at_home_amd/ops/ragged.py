@@ -107,12 +107,17 @@ def ragged_ungather(y: torch.Tensor, layout: RaggedLayout) -> torch.Tensor:
     return ragged_combine(y, RaggedLayout(layout.offsets, layout.order, rows), weights)
 
 
-def ragged_combine(y: torch.Tensor, layout: RaggedLayout, weights: torch.Tensor) -> torch.Tensor:
+def ragged_combine(y: torch.Tensor, layout: RaggedLayout, weights: torch.Tensor,
+                   min_mass: float = 0.0) -> torch.Tensor:
     """y [T * k, D] -> [T, D], each token's rows by its weights [T, k], which are
-    normalised over the slots that have a row (functional.combine). On a GPU: y
+    normalised over the slots that have a row: divided by their sum, or by
+    min_mass where that is larger (the bound on 1 / sum that functional.combine
+    has behind a capacity, 0.2). A sum of zero or less gives zeros. On a GPU: y
     bf16, D a multiple of 8, weights fp32."""
     from .functional import combine
 
+    if not min_mass >= 0:
+        raise ValueError(f"min_mass must not be negative, got {min_mass}")
     _check_layout(layout, y, "y")
     if y.dim() != 2 or y.shape[0] != layout.order.numel():
         raise ValueError(f"y must be [{layout.order.numel()}, D], the layout's rows, got {tuple(y.shape)}")
@@ -126,7 +131,9 @@ def ragged_combine(y: torch.Tensor, layout: RaggedLayout, weights: torch.Tensor)
             raise ValueError(f"weights must be fp32, got {weights.dtype}")
         y = _ready(y)
     one = torch.zeros_like(layout.rows)
-    return combine(y.unsqueeze(0), one, layout.rows, weights, layout.order.unsqueeze(0))
+    # the least mass is fp32's smallest normal number, whose inverse is finite
+    return combine(y.unsqueeze(0), one, layout.rows, weights, layout.order.unsqueeze(0),
+                   max(min_mass, torch.finfo(torch.float32).tiny))
 
 
 # ---------------------------------------------------------------------------

@@ -732,7 +732,8 @@ class ExpertParallelMoE(nn.Module):
         else:
             y = self._dropless_sharded(rows, counts, tm)
         with tm("moe_combine"):
-            return Fops.ragged_combine(y, layout, topk_w), counts
+            # as behind a capacity: where experts have left, few weights may be left over
+            return Fops.ragged_combine(y, layout, topk_w, min_mass=0.2), counts
 
     def _dropless_sharded(self, rows: torch.Tensor, counts: torch.Tensor, tm) -> torch.Tensor:
         """The FFN where experts are spread over ranks. Rows are sorted by expert,

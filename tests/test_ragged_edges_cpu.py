@@ -46,6 +46,7 @@ class TestRowsRefuse:
         (dict(weights=torch.ones(6)), "weights must be"),
         (dict(weights=torch.ones(3, 2, device="meta")), "one device"),
         (dict(layout=layout._replace(order=layout.order[:4])), "order"),
+        (dict(min_mass=-0.1), "min_mass"),
     ])
     def test_combine(self, change, match):
         with pytest.raises(ValueError, match=match):
@@ -62,6 +63,29 @@ class TestRowsRefuse:
     def test_what_the_kernels_do_not_take(self, t, match):
         with pytest.raises(ValueError, match=match):
             ragged._check_gpu_rows(t, "x")
+
+
+def test_weights_of_little_mass():
+    """However small the weights are together, they are normalised; min_mass bounds that."""
+    layout = layout_of([[0, 1], [1, 2], [-1, 2], [0, 2], [-1, -1], [2, 0]], 3)
+    y = torch.randn(12, 8, dtype=torch.double, requires_grad=True)
+    w = torch.tensor([[0.05, 0.05], [1e-3, 3e-3], [0.9, 0.02], [1e-30, 1e-30], [0.5, 0.5], [0.7, 0.3]],
+                     dtype=torch.double, requires_grad=True)
+    there = (layout.rows >= 0).double()
+    dy = torch.randn(6, 8, dtype=torch.double)
+    for least in (0.0, 0.2):
+        mass = (w * there).sum(1, keepdim=True)
+        share = w * there / torch.where(mass > 0, mass.clamp(min=least), 1.0)
+        want = (share[..., None] * y[layout.rows.clamp(min=0).long()]).sum(1)
+        got = Fops.ragged_combine(y, layout, w, min_mass=least)
+        assert torch.allclose(got, want, rtol=1e-14, atol=1e-14)
+        for a, b in zip(torch.autograd.grad(got, (y, w), dy), torch.autograd.grad(want, (y, w), dy)):
+            # dots of 8 products in fp32, 8 * 2^-24 of sums of sizes below 30, over the mass
+            assert ((a - b).abs() <= 30 * 8 * 2.0 ** -24 / mass.detach().clamp(min=1e-30) if a.shape == w.shape
+                    else (a - b).abs() <= 1e-14).all()
+    ones = torch.ones(12, 8)
+    out = Fops.ragged_combine(ones, layout, w.detach().float())
+    assert torch.allclose(out[[0, 1, 2, 3, 5]], ones[:5], rtol=2.0 ** -22) and not out[4].any()
 
 
 @pytest.mark.parametrize("dropless", [False, True])

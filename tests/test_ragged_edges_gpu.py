@@ -73,6 +73,45 @@ def test_rows_from_views():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("least", [0.0, 0.2])
+@pytest.mark.parametrize("D", [8, 24, 1032])
+def test_weights_of_little_mass(D, least):
+    """However small the weights are together, they are normalised; min_mass bounds that."""
+    g = torch.Generator().manual_seed(D)
+    T, k = 60, 4
+    ids = torch.randint(0, 9, (T, k), generator=g).int()
+    ids[torch.rand(T, k, generator=g) < 0.3] = -1
+    ids[7] = -1
+    layout = Fops.ragged_layout(ids.to(DEV), 9)
+    w = torch.rand(T, k, generator=g) * 10.0 ** -torch.arange(T)[:, None].div(2, rounding_mode="floor")  # down to 1e-29
+    w = w.to(DEV).requires_grad_(True)
+    y = torch.randn(T * k, D, generator=g).bfloat16().to(DEV).requires_grad_(True)
+    dy = torch.randn(T, D, generator=g).bfloat16().to(DEV)
+    out = Fops.ragged_combine(y, layout, w, min_mass=least)
+    dyy, dw = torch.autograd.grad(out, (y, w), dy)
+    yd, wd = y.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+    there = (layout.rows >= 0).double()
+    mass = (wd * there).sum(1, keepdim=True)
+    div = torch.where(mass > 0, mass.clamp(min=least), 1.0)
+    share = wd * there / div
+    rows = yd[layout.rows.clamp(min=0).long()]
+    want = (share[..., None] * rows).sum(1)
+    dyy64, dw64 = torch.autograd.grad(want, (yd, wd), dy.double())
+    # shares: a sum of 4, an inverse and a product in fp32; then k products and sums; one rounding to bf16
+    part = 16 * 2.0 ** -24
+    with torch.no_grad():
+        size = (share[..., None] * rows.abs()).sum(1)
+        assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + part * size + 1e-30).all()
+        assert ((dyy.double() - dyy64).abs() <= (2.0 ** -8 + part) * 1.01 * dyy64.abs() + 1e-30).all()
+        # <dy, y_j> - <dy, y> with y as it was rounded, over the mass
+        a = dy.double().abs()
+        dots = (a[:, None] * rows.abs()).sum(-1) + (a * want.abs()).sum(-1, keepdim=True)
+        tol = (2.0 ** -8 * 1.01 * (a * want.abs()).sum(-1, keepdim=True) + (D + 16) * 2.0 ** -24 * dots) / div
+        assert torch.isfinite(dw).all()
+        assert ((dw.double() - dw64).abs() <= (tol + part * dw64.abs()) * there + 1e-30).all()
+    assert not out[7].any() and not dw[7].any()
+
+
 class TestNoTokens:
     def make_stack(self):
         torch.manual_seed(0)
