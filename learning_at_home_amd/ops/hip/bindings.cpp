@@ -78,6 +78,11 @@ hipStream_t cur_stream() { return at::hip::getCurrentHIPStream().stream(); }
     TORCH_CHECK(err == hipSuccess, "launch: ", hipGetErrorString(err));     \
   } while (0)
 
+// The kernels have no forward-mode derivative: a tangent would be lost without a word.
+bool has_tangent(const torch::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+#define CHECK_NO_TANGENT(t, name) \
+  TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), name " has no forward-mode derivative on the GPU")
+
 // contiguous, from a multiple of 16 bytes on: what the kernels load
 torch::Tensor ready(const torch::Tensor& t) {
   const auto c = t.contiguous();
@@ -453,6 +458,7 @@ std::vector<torch::Tensor> flash_attn_bwd(torch::Tensor q, torch::Tensor k,
 
 static void check_ragged(const torch::Tensor& a, const torch::Tensor& b,
                          const torch::Tensor& offsets) {
+  CHECK_NO_TANGENT(a, "a product by groups");  // ragged_ffn's
   for (const auto* t : {&a, &b}) {
     CHECK_CUDA(*t); CHECK_BF16(*t); CHECK_CONTIG(*t); CHECK_ALIGNED(*t);
   }
@@ -672,6 +678,8 @@ struct GroupedLinear : public torch::autograd::Function<GroupedLinear> {
 
 torch::Tensor grouped_linear(torch::Tensor x, torch::Tensor w, torch::Tensor offsets,
                              c10::optional<torch::Tensor> bias, c10::optional<std::string> activation) {
+  for (const auto* t : {&x, &w}) CHECK_NO_TANGENT(*t, "grouped_linear");
+  if (bias.has_value()) CHECK_NO_TANGENT(*bias, "grouped_linear");
   TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 3 && x.size(1) == w.size(2),
                     "x must be [R, K] and weight [E, N, K], got ", x.sizes(), " and ", w.sizes());
   TORCH_CHECK_VALUE(offsets.scalar_type() == at::kInt && offsets.dim() == 1 &&
@@ -720,16 +728,20 @@ struct ClipList {
   std::vector<long> n;
   std::vector<int> kind;
   bool taken = true;  // all on one GPU, of kinds and layouts that the kernels take
+  bool tangent = false;
   explicit ClipList(const std::vector<torch::Tensor>& ts) {
     TORCH_CHECK_VALUE(!ts.empty(), "no tensors");
     p.reserve(ts.size()); n.reserve(ts.size()); kind.reserve(ts.size());
     for (const auto& t : ts) {
       const int k = clip_kind(t);
       taken = taken && t.is_cuda() && t.device() == ts[0].device() && k >= 0 && t.is_contiguous();
+      tangent = tangent || has_tangent(t);
       p.push_back(t.data_ptr());
       n.push_back(t.numel());
       kind.push_back(k);
     }
+    TORCH_CHECK_NOT_IMPLEMENTED(!(taken && tangent), "gradient norms, clipping and steps have no forward-mode "
+                                                     "derivative on the GPU");
   }
 };
 

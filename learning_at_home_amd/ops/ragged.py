@@ -185,7 +185,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     gradients. Sums are fp32; y, dx and dW are rounded once (with gelu the
     gradient at its input is rounded to bf16 between the products). On a GPU: bf16,
     at most 4096 groups, N and K multiples of 8 below 2^21, N * K below 2^30.
-    Differentiable once. As with other operators, a backward pass is captured into
+    Differentiable once, backwards: on a GPU forward-mode derivatives and a
+    backward pass with create_graph=True are refused. As with other operators, a backward pass is captured into
     a graph with torch.autograd.grad or with no eager graph of the leaves alive."""
     if x.is_cuda and HAS_HIP:  # checks, gradients and all: bindings.cpp
         return _C.grouped_linear(x, weight, offsets, bias, activation)

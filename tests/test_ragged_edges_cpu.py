@@ -5,9 +5,11 @@ import socket
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 import torch.distributed as dist
 import torch.multiprocessing as mp
 
+from learning_at_home_amd.ops import _C
 from learning_at_home_amd.ops import functional as Fops
 from learning_at_home_amd.ops import ragged
 from learning_at_home_amd.parallel import ExpertParallelMoE
@@ -131,3 +133,17 @@ def test_idle_rank_over_gloo():
         p.join(60)
     assert got[0] == (7, 7, 14, True)
     assert got[1][:3] == (0, 0, 0) and not got[1][3]
+
+
+def test_kernels_refuse_tangents():
+    """What the products' entry says of a dual tensor, before it looks where that is."""
+    x, w = torch.zeros(4, 8).bfloat16(), torch.zeros(2, 16, 8).bfloat16()
+    off, b = torch.tensor([0, 1, 4], dtype=torch.int32), torch.zeros(2, 16)
+    with fwd.dual_level():
+        for i in range(3):
+            args = [x, w, b]
+            args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                _C.grouped_linear(args[0], args[1], off, args[2])
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            _C.ragged_nt(fwd.make_dual(x, x), w, off)

@@ -2,6 +2,7 @@
 together, no tokens, weights of little mass, derivatives that the operators do not have."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 pytestmark = pytest.mark.gpu
 
@@ -162,3 +163,27 @@ class TestNoTokens:
         assert x.grad.shape == (0, 128) and not moe.gate.weight.grad.any()
         moe(torch.randn(3, 128, device=DEV).bfloat16())  # no error was left behind
         torch.cuda.synchronize()
+
+
+class TestDerivativesThatAreNotThere:
+    def test_forward_mode(self):
+        """A tangent is refused, not dropped; the CPU's plain torch keeps it."""
+        torch.manual_seed(0)
+        stack = ExpertStack(2, 128, 256).to(DEV)
+        stack.init_gpu_state()
+        x, w = torch.randn(4, 128, device=DEV).bfloat16(), torch.randn(2, 16, 128, device=DEV).bfloat16()
+        b = torch.randn(2, 16, device=DEV)
+        off = torch.tensor([0, 1, 4], dtype=torch.int32, device=DEV)
+        layout = Fops.ragged_layout(torch.tensor([[0], [1], [1], [1]], dtype=torch.int32, device=DEV), 2)
+        with fwd.dual_level():
+            def dual(t):
+                return fwd.make_dual(t, torch.ones_like(t))
+
+            for call in (lambda: Fops.grouped_linear(dual(x), w, off), lambda: Fops.grouped_linear(x, dual(w), off),
+                         lambda: Fops.grouped_linear(x, w, off, dual(b)), lambda: Fops.ragged_ffn(dual(x), off, stack),
+                         lambda: Fops.ragged_gather(dual(x), layout),
+                         lambda: Fops.ragged_combine(x, layout, dual(torch.ones(4, 1, device=DEV))),
+                         lambda: Fops.grad_clip_scale([dual(b)], 1.0), lambda: Fops.clip_grad_norm_([b, dual(b.clone())], 1.0)):
+                with pytest.raises(NotImplementedError, match="forward"):
+                    call()
+        Fops.grouped_linear(x, w, off, b)
