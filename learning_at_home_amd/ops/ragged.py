@@ -11,7 +11,8 @@ the groups as they are:
     out = ragged_combine(y, layout, topk_w)        # [T*k, D] -> [T, D]
 
 Nothing waits for the host, so a forward, a backward or a single decoded token
-can be captured in a graph. Slots whose id is no expert (padding, experts that
+can be captured in a graph. The kernels' gradients cannot be differentiated
+again: that raises an error. Slots whose id is no expert (padding, experts that
 left) have no row; rows from offsets[E] on belong to nobody: products give
 zeros there, and weights get nothing from them.
 
@@ -24,7 +25,6 @@ from typing import NamedTuple, Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from . import _C, HAS_HIP
 
@@ -63,6 +63,52 @@ def ragged_layout(topk_idx: torch.Tensor, num_experts: int) -> RaggedLayout:
                         torch.where(key < num_experts, rows, -1).int().view(topk_idx.shape))
 
 
+class _Refuse(torch.autograd.Function):
+    """A gradient as it is. The kernels know nothing of the tensors `of` that it depends on, so
+    a second derivative would silently lack this path: it raises an error instead."""
+
+    @staticmethod
+    def forward(ctx, grad, *of):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("the ragged operators are differentiable once on the GPU")
+
+
+def _once(grad, *of):
+    return _Refuse.apply(grad, *of) if torch.is_grad_enabled() and grad is not None else grad
+
+
+class _GatherHip(torch.autograd.Function):
+    """Rows by the kernels of the capacity layout, all in one group: their number is their slot."""
+
+    @staticmethod
+    def forward(ctx, x, rows, order):
+        ctx.save_for_backward(rows)
+        return _C.dispatch_gather(x, order.unsqueeze(0), rows.shape[1])[0]
+
+    @staticmethod
+    def backward(ctx, d):
+        rows, = ctx.saved_tensors
+        return _once(_C.dispatch_bwd(d.unsqueeze(0), torch.zeros_like(rows), rows, rows.shape[0]), d), None, None
+
+
+class _CombineHip(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, rows, order, w, least):
+        out = _C.combine_fwd(y.unsqueeze(0), torch.zeros_like(rows), rows, w, least)
+        ctx.save_for_backward(y, out, rows, order, w)
+        ctx.least = least
+        return out
+
+    @staticmethod
+    def backward(ctx, d):
+        y, out, rows, order, w = ctx.saved_tensors
+        dy, dw = _C.combine_bwd(d, y.unsqueeze(0), out, torch.zeros_like(rows), rows, w, order.unsqueeze(0), ctx.least)
+        return _once(dy[0], w, d), None, None, _once(dw, y, w, d), None
+
+
 def _check_layout(layout, t, name):
     """The layout's parts go together, and with t: the kernels take rows and slots from them."""
     rows, order = layout.rows, layout.order
@@ -93,7 +139,7 @@ def ragged_gather(x: torch.Tensor, layout: RaggedLayout) -> torch.Tensor:
         raise ValueError(f"x must be [{T}, D], a row for each token of the layout, got {tuple(x.shape)}")
     if x.is_cuda and HAS_HIP:
         _check_gpu_rows(x, "x")
-        x = _ready(x)
+        return _GatherHip.apply(_ready(x), layout.rows, layout.order)
     one = torch.zeros_like(layout.rows)  # all rows in one group: their number is their slot
     return dispatch(x, one, layout.rows, layout.order.unsqueeze(0), k)[0]
 
@@ -118,6 +164,7 @@ def ragged_combine(y: torch.Tensor, layout: RaggedLayout, weights: torch.Tensor,
 
     if not min_mass >= 0:
         raise ValueError(f"min_mass must not be negative, got {min_mass}")
+    least = max(min_mass, torch.finfo(torch.float32).tiny)  # the smallest normal number's inverse is finite
     _check_layout(layout, y, "y")
     if y.dim() != 2 or y.shape[0] != layout.order.numel():
         raise ValueError(f"y must be [{layout.order.numel()}, D], the layout's rows, got {tuple(y.shape)}")
@@ -129,11 +176,9 @@ def ragged_combine(y: torch.Tensor, layout: RaggedLayout, weights: torch.Tensor,
         _check_gpu_rows(y, "y")
         if weights.dtype != torch.float32:
             raise ValueError(f"weights must be fp32, got {weights.dtype}")
-        y = _ready(y)
+        return _CombineHip.apply(_ready(y), layout.rows, layout.order, weights, least)
     one = torch.zeros_like(layout.rows)
-    # the least mass is fp32's smallest normal number, whose inverse is finite
-    return combine(y.unsqueeze(0), one, layout.rows, weights, layout.order.unsqueeze(0),
-                   max(min_mass, torch.finfo(torch.float32).tiny))
+    return combine(y.unsqueeze(0), one, layout.rows, weights, layout.order.unsqueeze(0), least)
 
 
 # ---------------------------------------------------------------------------
@@ -223,7 +268,6 @@ class _RaggedFFNHip(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
         from .functional import _wait_pending_opt
 
@@ -238,7 +282,7 @@ class _RaggedFFNHip(torch.autograd.Function):
         _C.ragged_tn(dh, x, offsets, stack.main_grad_W1, stack.main_grad_b1, acc)
         _C.ragged_tn(dy, h, offsets, stack.main_grad_W2, stack.main_grad_b2, acc)
         stack.grad_ready = True
-        return dx, None, None
+        return _once(dx, x, dy), None, None
 
 
 def _check_stack(stack):

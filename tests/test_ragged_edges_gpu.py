@@ -187,3 +187,32 @@ class TestDerivativesThatAreNotThere:
                 with pytest.raises(NotImplementedError, match="forward"):
                     call()
         Fops.grouped_linear(x, w, off, b)
+
+    @pytest.mark.parametrize("what", ["gather", "ungather", "combine", "ffn"])
+    def test_second_derivatives(self, what):
+        """With create_graph=True the gradients are the same, and refuse to be differentiated."""
+        torch.manual_seed(0)
+        stack = ExpertStack(2, 128, 256).to(DEV)
+        stack.init_gpu_state()
+        layout = Fops.ragged_layout(torch.tensor([[0, 1], [1, -1], [1, 0]], dtype=torch.int32, device=DEV), 2)
+        T = 3 if what == "gather" else 6
+        x = torch.randn(T, 128, device=DEV).bfloat16().requires_grad_(True)
+        w = torch.rand(3, 2, device=DEV, requires_grad=True)
+
+        def call(x, w):
+            return {"gather": lambda: Fops.ragged_gather(x, layout), "ungather": lambda: Fops.ragged_ungather(x, layout),
+                    "combine": lambda: Fops.ragged_combine(x, layout, w),
+                    "ffn": lambda: Fops.ragged_ffn(x, layout.offsets, stack)}[what]()
+
+        leaves = (x, w) if what == "combine" else (x,)
+        y = call(x, w)
+        dy = torch.randn_like(y).requires_grad_(True)
+        plain = torch.autograd.grad(call(x, w), leaves, dy)
+        grads = torch.autograd.grad(call(x, w), leaves, dy, create_graph=True)
+        for a, b in zip(plain, grads):
+            assert torch.equal(a, b) and b.requires_grad
+            with pytest.raises(RuntimeError, match="once"):
+                torch.autograd.grad(b.float().square().sum(), dy, retain_graph=True)
+            if what != "gather" and what != "ungather":  # linear: nothing of x in its gradient
+                with pytest.raises(RuntimeError, match="once"):
+                    torch.autograd.grad(b.float().square().sum(), leaves[-1], retain_graph=True)
