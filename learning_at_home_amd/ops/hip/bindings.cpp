@@ -52,7 +52,9 @@ int lah_ragged_parts(long, int, int, int, bool);
 long lah_ragged_tn_work(long, int, int, int);
 void lah_ragged_tn(const void*, const void*, void*, void*, int, const void*, long, int, int,
                    int, int, void*, hipStream_t);
-void lah_ragged_slope(const void*, const void*, void*, long, hipStream_t);
+long lah_ragged_slope_work(long, int, int);
+void lah_ragged_slope(const void*, const void*, void*, void*, int, const void*, long, int, int, void*,
+                      hipStream_t);
 long lah_clip_partials(int);
 void lah_grad_norm(void* const*, const long*, const int*, int, void*, float, float, void*,
                    void*, hipStream_t);
@@ -624,16 +626,35 @@ void ragged_tn(torch::Tensor d, torch::Tensor x, torch::Tensor offsets, torch::T
   CHECK_LAUNCH();
 }
 
-// dP = dy * der
-torch::Tensor ragged_slope(torch::Tensor dy, torch::Tensor der) {
-  CHECK_CUDA(dy); CHECK_BF16(dy); CHECK_CONTIG(dy); CHECK_ALIGNED(dy);
+// dP = dy * der in bf16 (if `write`; rows of nobody are left as they are), and db[e], if given,
+// its sums over the rows of e before the rounding
+torch::Tensor ragged_slope(torch::Tensor dy, torch::Tensor der, torch::Tensor offsets,
+                           c10::optional<torch::Tensor> db, bool write) {
+  check_ragged(dy, dy, offsets);
   check_slope(der);
-  TORCH_CHECK(dy.sizes() == der.sizes() && dy.device() == der.device() && dy.numel() % 8 == 0,
-              "dy and der must go together");
+  TORCH_CHECK(dy.sizes() == der.sizes() && dy.device() == der.device() && dy.size(1) % 8 == 0 &&
+              dy.size(1) < 1 << 21, "dy and der must be [R, N], N a multiple of 8");
+  TORCH_CHECK(write || db.has_value(), "nothing is asked for");
+  const int64_t R = dy.size(0), N = dy.size(1), E = offsets.numel() - 1;
+  TORCH_CHECK(E <= 65535, "too many groups");
+  void* db_p = nullptr;
+  int db_bf16 = 0;
+  if (db.has_value()) {
+    CHECK_CONTIG(*db);
+    db_bf16 = db->scalar_type() == at::kBFloat16;
+    TORCH_CHECK(db_bf16 || db->scalar_type() == at::kFloat, "db must be bf16 or fp32");
+    TORCH_CHECK(db->dim() == 2 && db->size(0) == E && db->size(1) == N && db->device() == dy.device(),
+                "db must be [E, N] on the GPU of dy");
+    db_p = db->data_ptr();
+  }
   ON_DEVICE_OF(dy);
-  auto dp = torch::empty_like(dy);
-  if (dy.numel() == 0) return dp;
-  lah_ragged_slope(dy.data_ptr(), der.data_ptr(), dp.data_ptr(), dy.numel(), cur_stream());
+  torch::Tensor dp, work;
+  if (write) dp = torch::empty_like(dy);
+  if (N == 0) return dp;
+  const long room = db.has_value() ? lah_ragged_slope_work(R, (int)E, (int)N) : 0;
+  if (room > 0) work = torch::empty({room}, dy.options().dtype(at::kFloat));
+  lah_ragged_slope(dy.data_ptr(), der.data_ptr(), ptr_or_null(dp), db_p, db_bf16, offsets.data_ptr(), R, (int)E,
+                   (int)N, ptr_or_null(work), cur_stream());
   CHECK_LAUNCH();
   return dp;
 }
@@ -661,14 +682,18 @@ struct GroupedLinear : public torch::autograd::Function<GroupedLinear> {
     const int64_t bias = ctx->saved_data["bias"].toInt();
     if (!grads[0].defined()) return {{}, {}, {}, {}, {}};
     auto d = ready(grads[0]);
-    if (der.defined()) d = ragged_slope(d, der);
     torch::Tensor dx, dw, db;
-    const bool want_w = ctx->needs_input_grad(1), want_b = bias >= 0 && ctx->needs_input_grad(2);
-    if (ctx->needs_input_grad(0)) dx = ragged_nn(d, w, offsets, c10::nullopt);
-    if (want_w || want_b) {
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+    c10::optional<torch::Tensor> b;
+    if (bias >= 0 && ctx->needs_input_grad(2))
+      b = db = torch::empty({w.size(0), w.size(1)}, w.options().dtype((at::ScalarType)bias));
+    if (der.defined()) {
+      if (want_x || want_w || db.defined()) d = ragged_slope(d, der, offsets, b, want_x || want_w);
+      b.reset();
+    }
+    if (want_x) dx = ragged_nn(d, w, offsets, c10::nullopt);
+    if (want_w || b.has_value()) {
       dw = torch::empty_like(w);
-      c10::optional<torch::Tensor> b;
-      if (want_b) b = db = torch::empty({w.size(0), w.size(1)}, w.options().dtype((at::ScalarType)bias));
       ragged_tn(d, x, offsets, dw, b, false);
       if (!want_w) dw = torch::Tensor();
     }
@@ -853,7 +878,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("db") = py::none(), py::arg("accumulate") = false);
   m.def("grouped_linear", &grouped_linear, py::arg("x"), py::arg("weight"), py::arg("offsets"),
         py::arg("bias") = py::none(), py::arg("activation") = py::none());
-  m.def("ragged_slope", &ragged_slope, py::arg("dy"), py::arg("der"));
+  m.def("ragged_slope", &ragged_slope, py::arg("dy"), py::arg("der"), py::arg("offsets"),
+        py::arg("db") = py::none(), py::arg("write") = true);
   m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("max_norm"), py::arg("eps") = 1e-6);
   m.def("grad_scale_", &grad_scale_, py::arg("grads"), py::arg("scale"));
   m.def("master_sgd_", &master_sgd_, py::arg("params"), py::arg("masters"), py::arg("grads"),

@@ -1566,22 +1566,112 @@ extern "C" void lah_ragged_tn(const void* d, const void* x, void* dw, void* db, 
   else launch_weights<R_F32>(a, table, stream);
 }
 
-// dP = dy * slope, rounded to bf16 for the two products that take it
-__launch_bounds__(256) __global__ void ragged_slope_kernel(const __bf16* __restrict__ dy,
-                                                           const _Float16* __restrict__ der,
-                                                           __bf16* __restrict__ dp, long n) {
-  for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long)gridDim.x * 2048) {
-    const bf16x8 y = *(const bf16x8*)(dy + i);
-    const f16x8 d = *(const f16x8*)(der + i);
-    bf16x8 o;
+// dP = dy * slope, rounded to bf16 for the two products that take it, and db, its sums over each
+// group's rows as they were before that. A block has up to 128 rows of one group by 256
+// columns, 8 a lane; where there are fewer columns its lanes take more rows. Its sums go to
+// part[slot], and are joined in the slots' order. Or it has a whole group, by 64 columns, and
+// needs no join. Rows of nobody are left out: nothing reads their dP. Bound by HBM: dy and the
+// slope in, dP out.
+enum { S_NONE = 0, S_PART = 1, S_GROUP = 2 };  // sums: none, of a tile, of a group
+template <bool WRITE, int SUMS>
+__launch_bounds__(256) __global__ void ragged_slope_kernel(RaggedArgs a, const __bf16* __restrict__ dy,
+                                                           __bf16* __restrict__ dp, float* __restrict__ part,
+                                                           int shift) {
+  __shared__ __attribute__((aligned(16))) float sums[2048];  // [row lanes][columns]
+  const int lanes = 1 << shift, NT = cdiv(a.N, lanes * 8), L = blockIdx.y * gridDim.x + blockIdx.x, slot = L / NT;
+  const int e = SUMS == S_GROUP ? slot : __builtin_amdgcn_readfirstlane(find_expert<RBM>(a.offsets, a.E, slot));
+  long lo, hi;
+  expert_rows(a, e, &lo, &hi);
+  const long row0 = SUMS == S_GROUP ? lo : lo + (long)(slot - (int)(lo / RBM) - e) * RBM;
+  if (e >= a.E || (SUMS != S_GROUP && (row0 < lo || row0 >= hi))) return;
+  const int rows = (int)(SUMS == S_GROUP ? hi - lo : min(hi - row0, (long)RBM)), c = threadIdx.x & (lanes - 1), r0 = threadIdx.x >> shift;
+  const int n0 = L % NT * lanes * 8, n = n0 + c * 8, step = 256 >> shift;
+  float sum[8] = {};
+  if (n < a.N) {
+    const long at = row0 * a.N + n;
+    for (int r = r0; r < rows; r += 4 * step) {  // four rows' loads at once
+      bf16x8 y[4];
+      f16x8 d[4];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) o[x] = f2bf(bf2f(y[x]) * (float)d[x]);
-    *(bf16x8*)(dp + i) = o;
+      for (int u = 0; u < 4; ++u) {
+        const bool in = r + u * step < rows;
+        y[u] = in ? *(const bf16x8*)(dy + at + (long)(r + u * step) * a.N) : bf16x8{};
+        d[u] = in ? *(const f16x8*)(a.der + at + (long)(r + u * step) * a.N) : f16x8{};
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        bf16x8 o;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const float v = bf2f(y[u][x]) * (float)d[u][x];
+          sum[x] += v;
+          o[x] = f2bf(v);
+        }
+        if (WRITE && r + u * step < rows) *(bf16x8*)(dp + at + (long)(r + u * step) * a.N) = o;
+      }
+    }
   }
+  if (SUMS == S_NONE) return;
+#pragma unroll
+  for (int h = 0; h < 8; h += 4)
+    *(f32x4*)(sums + (r0 * lanes + c) * 8 + h) = f32x4{sum[h], sum[h + 1], sum[h + 2], sum[h + 3]};
+  __syncthreads();
+  const int col = threadIdx.x;
+  if (col >= lanes * 8 || n0 + col >= a.N) return;
+  float all = 0.f;
+  for (int r = 0; r < step; ++r) all += sums[r * lanes * 8 + col];
+  const long to = (long)slot * a.N + n0 + col;
+  if (SUMS == S_PART) part[to] = all;
+  else if (a.bias_bf16) ((__bf16*)a.db)[to] = f2bf(all);
+  else ((float*)a.db)[to] = all;
 }
 
-extern "C" void lah_ragged_slope(const void* dy, const void* der, void* dp, long n, hipStream_t stream) {
-  const long blocks = (n / 8 + 255) / 256;
-  hipLaunchKernelGGL(ragged_slope_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, stream,
-                     (const __bf16*)dy, (const _Float16*)der, (__bf16*)dp, n);
+// db of each group from its slots' sums: four quarters of the slots in turn, joined in order
+__launch_bounds__(256) __global__ void ragged_join_sums_kernel(RaggedArgs a, const float* __restrict__ part) {
+  __shared__ float sums[4][64];
+  const int e = blockIdx.y, c = threadIdx.x & 63, q = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
+  long lo, hi;
+  expert_rows(a, e, &lo, &hi);
+  const int count = (int)((hi - lo + RBM - 1) / RBM);
+  float sum = 0.f;
+  if (n < a.N) {
+    const float* at = part + ((lo / RBM) + e) * a.N + n;
+#pragma unroll 8
+    for (int i = q; i < count; i += 4) sum += at[(long)i * a.N];
+  }
+  sums[q][c] = sum;
+  __syncthreads();
+  if (q > 0 || n >= a.N) return;
+  const float all = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+  const long to = (long)e * a.N + n;
+  if (a.bias_bf16) ((__bf16*)a.db)[to] = f2bf(all);
+  else ((float*)a.db)[to] = all;
+}
+
+// Whole groups where none can be long: 128 rows are a round of a block, and one more launch is
+// as long as a few. 12 groups of 1998 rows, 136 -> 328, forward and backward: 80 us so, 86 joined.
+static bool slope_by_group(long R) { return R <= 16 * RBM; }
+
+// fp32 numbers that the slots' sums need room for
+extern "C" long lah_ragged_slope_work(long R, int E, int N) {
+  return slope_by_group(R) ? 0 : (R / RBM + E + 1) * N;
+}
+
+// dp [R, N] = dy * der, or null; db [E, N] or null, with work: lah_ragged_slope_work numbers
+extern "C" void lah_ragged_slope(const void* dy, const void* der, void* dp, void* db, int db_bf16,
+                                 const void* offsets, long R, int E, int N, void* work, hipStream_t stream) {
+  RaggedArgs a{nullptr, nullptr, nullptr, (const int*)offsets, nullptr, (_Float16*)der,
+               db, R, E, N, 0, 0, db_bf16, 1, false};
+  const bool by_group = db != nullptr && slope_by_group(R);
+  int shift = 0;
+  while (shift < (by_group ? 3 : 5) && (8 << shift) < N) ++shift;
+  const long tiles = by_group ? E : R / RBM + E + 1, blocks = tiles * cdiv(N, 8 << shift);
+  const unsigned wide = (unsigned)(blocks < 1 << 22 ? blocks : 1 << 22);  // 2^32 threads a dimension
+  auto kernel = dp == nullptr ? (by_group ? ragged_slope_kernel<false, S_GROUP> : ragged_slope_kernel<false, S_PART>)
+                : db == nullptr ? ragged_slope_kernel<true, S_NONE>
+                : by_group ? ragged_slope_kernel<true, S_GROUP> : ragged_slope_kernel<true, S_PART>;
+  hipLaunchKernelGGL(kernel, dim3(wide, (unsigned)((blocks + wide - 1) / wide)), dim3(256), 0, stream, a,
+                     (const __bf16*)dy, (__bf16*)dp, (float*)work, shift);
+  if (db != nullptr && !by_group)
+    hipLaunchKernelGGL(ragged_join_sums_kernel, dim3(cdiv(N, 64), E), dim3(256), 0, stream, a, (const float*)work);
 }

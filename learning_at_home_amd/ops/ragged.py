@@ -227,8 +227,9 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     R (a RaggedLayout's, or any other groups); bias [E, N]; activation None or
     "gelu" (its tanh form). Returns [R, N], zeros from row offsets[E] on.
     Differentiable in x, weight and bias; a group without rows has zero weight
-    gradients. Sums are fp32; y, dx and dW are rounded once (with gelu the
-    gradient at its input is rounded to bf16 between the products). On a GPU: bf16,
+    gradients. Sums are fp32; y, dx and dW are rounded once (with gelu its slope
+    is kept in fp16, and the gradient at its input is rounded to bf16 between the
+    products, not for the bias's sums). On a GPU: bf16,
     at most 4096 groups, N and K multiples of 8 below 2^21, N * K below 2^30.
     Differentiable once, backwards: on a GPU forward-mode derivatives and a
     backward pass with create_graph=True are refused. As with other operators, a backward pass is captured into
@@ -276,7 +277,8 @@ class _RaggedFFNHip(torch.autograd.Function):
         _check_stack(stack)
         _wait_pending_opt(stack)
         dy = _ready(dy)
-        dh = _C.ragged_nn(dy, stack.W2c, offsets, der)  # at gelu's input, rounded to bf16 for the next two products
+        dh = _C.ragged_nn(dy, stack.W2c, offsets, der)  # at gelu's input, rounded to bf16 for the next two
+        # products, and for b1's sums, which ride in one of them (as the capacity layout has them)
         dx = _C.ragged_nn(dh, stack.W1c, offsets) if ctx.needs_input_grad[0] else None
         acc = stack.grad_ready
         _C.ragged_tn(dh, x, offsets, stack.main_grad_W1, stack.main_grad_b1, acc)

@@ -113,6 +113,46 @@ def test_weights_of_little_mass(D, least):
     assert not out[7].any() and not dw[7].any()
 
 
+class TestBiasGradient:
+    @pytest.mark.parametrize("counts", [[1, 0, 2, 3, 1], [0, 0, 700, 128, 129, 127], [40000, 1, 0, 300], [0, 0], [1] * 600],
+                             ids=["few", "tiles", "long", "none", "many"])
+    @pytest.mark.parametrize("N", [8, 40, 136, 264, 2056])
+    @pytest.mark.parametrize("bias", [torch.float32, torch.bfloat16])
+    def test_sums_before_the_rounding(self, counts, N, bias):
+        """Behind gelu, db adds what dx and dW take rounded to bf16: here within fp32 and the slope's fp16."""
+        K, E, R = 8, len(counts), sum(counts) + 7
+        g = torch.Generator(device=DEV).manual_seed(N + R)
+        x = torch.randn(R, K, device=DEV, generator=g).bfloat16()
+        w = torch.randn(E, N, K, device=DEV, generator=g).bfloat16()
+        b = torch.randn(E, N, device=DEV, generator=g).to(bias)
+        dy = torch.randn(R, N, device=DEV, generator=g).bfloat16()
+        offsets = torch.nn.functional.pad(torch.tensor(counts, device=DEV).cumsum(0), (1, 0)).int()
+        x[offsets[-1]:], dy[offsets[-1]:] = float("nan"), float("inf")  # rows of nobody
+
+        def grads(which):
+            leaves = [t.detach().clone().requires_grad_(n in which) for n, t in (("x", x), ("w", w), ("b", b))]
+            y = Fops.grouped_linear(leaves[0], leaves[1], offsets, leaves[2], "gelu")
+            return dict(zip(which, torch.autograd.grad(y, [t for t in leaves if t.requires_grad], dy)))
+
+        full = grads("xwb")
+        at = offsets.tolist()
+        for e in range(E) if E < 100 else range(0, E, 97):
+            s = slice(at[e], at[e + 1])
+            xd, wd, n = x[s].double(), w[e].double(), at[e + 1] - at[e]
+            u = (xd @ wd.t() + b[e].double()).requires_grad_(True)
+            dp, = torch.autograd.grad(torch.nn.functional.gelu(u, approximate="tanh"), u, dy[s].double())
+            off = (K + 2) * 2.0 ** -23 * (xd.abs() @ wd.abs().t() + b[e].double().abs())
+            # the slope: fp16 (2^-11 of it, 2^-25 below its normal range), its argument's error (its own slope
+            # is at most 1), exp2 and reciprocal; then n products and sums in fp32; the result's own rounding
+            tol = (2.0 ** -11 * dp.abs() + dy[s].double().abs() * (off + 2.0 ** -20)).sum(0) * 1.01
+            tol = tol + (n + 1) * 2.0 ** -24 * dp.abs().sum(0) + torch.finfo(bias).eps / 2 * dp.sum(0).abs()
+            assert ((full["b"][e].double() - dp.sum(0)).abs() <= tol * 1.01 + 1e-30).all()
+        for which in ("b", "xb", "wb", "xw"):
+            got = grads(which)
+            for n in which:
+                assert torch.equal(got[n], full[n]), (which, n)
+
+
 class TestNoTokens:
     def make_stack(self):
         torch.manual_seed(0)
