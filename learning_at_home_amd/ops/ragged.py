@@ -243,11 +243,12 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
 def _grouped_linear_torch(x, weight, offsets, bias, gelu):
     at = offsets.tolist()
     parts = []
+    wide = torch.promote_types(x.dtype, torch.float32)  # sums, bias and gelu; rounded once
     for e, (lo, hi) in enumerate(zip(at[:-1], at[1:])):
-        h = x[lo:hi] @ weight[e].t()
+        h = x[lo:hi].to(wide) @ weight[e].to(wide).t()
         if bias is not None:
-            h = h + bias[e].to(h.dtype)
-        parts.append(F.gelu(h, approximate="tanh") if gelu else h)
+            h = h + bias[e].to(wide)
+        parts.append((F.gelu(h, approximate="tanh") if gelu else h).to(x.dtype))
     parts.append(x.new_zeros(x.shape[0] - at[-1], weight.shape[1]))
     return torch.cat(parts)
 

@@ -135,6 +135,39 @@ def test_idle_rank_over_gloo():
     assert got[1][:3] == (0, 0, 0) and not got[1][3]
 
 
+@pytest.mark.parametrize("bias", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("activation", [None, "gelu"])
+def test_low_precision_is_rounded_once(activation, bias):
+    """bf16 products on the CPU: fp32 sums and bias, one rounding of each result, as on the GPU."""
+    g = torch.Generator().manual_seed(0)
+    K, N, counts = 24, 40, [3, 0, 50, 1]
+    off = torch.tensor([0, 3, 3, 53, 54], dtype=torch.int32)
+    x, w = torch.randn(56, K, generator=g).bfloat16(), torch.randn(4, N, K, generator=g).bfloat16()
+    b, dy = torch.randn(4, N, generator=g).to(bias), torch.randn(56, N, generator=g).bfloat16()
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = Fops.grouped_linear(leaves[0], leaves[1], off, leaves[2], activation)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    assert y.dtype == dx.dtype == dw.dtype == torch.bfloat16 and db.dtype == bias
+    half, at = 2.0 ** -8, off.tolist()
+    for e, n in enumerate(counts):
+        s = slice(at[e], at[e + 1])
+        xd, wd, d = x[s].double(), w[e].double(), dy[s].double()
+        u = (xd @ wd.t() + b[e].double()).requires_grad_(True)
+        v = torch.nn.functional.gelu(u, approximate="tanh") if activation else u * 1
+        dp, = torch.autograd.grad(v, u, d)
+        # a sum of K products and the bias in fp32, gelu's slope at most 1.13 and its own 2^-20 of fp32's tanh
+        off_u = (K + 2) * 2.0 ** -24 * (xd.abs() @ wd.abs().t() + b[e].double().abs())
+        soft = 2.0 ** -20 if activation else 0.0
+        assert ((y[s].double() - v).abs() <= half * v.abs() + 1.13 * off_u + soft * u.abs() + 1e-30).all()
+        # dP: dy times the slope, whose own slope is at most 1
+        off_p = d.abs() * ((off_u + 4 * soft) if activation else 0 * off_u)
+        for got, want, size in ((dx[s], dp @ wd, off_p @ wd.abs() + (N + 1) * 2.0 ** -24 * dp.abs() @ wd.abs()),
+                                (dw[e], dp.t() @ xd, off_p.t() @ xd.abs() + (n + 1) * 2.0 ** -24 * dp.abs().t() @ xd.abs()),
+                                (db[e], dp.sum(0), off_p.sum(0) + (n + 1) * 2.0 ** -24 * dp.abs().sum(0))):
+            assert ((got.double() - want).abs() <= torch.finfo(got.dtype).eps / 2 * want.abs() + 1.01 * size + 1e-30).all()
+    assert not y[54:].any() and not dx[54:].any()
+
+
 def test_kernels_refuse_tangents():
     """What the products' entry says of a dual tensor, before it looks where that is."""
     x, w = torch.zeros(4, 8).bfloat16(), torch.zeros(2, 16, 8).bfloat16()
