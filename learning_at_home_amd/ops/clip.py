@@ -41,7 +41,7 @@ def grad_clip_scale(tensors: Sequence[torch.Tensor], max_norm: float,
             return tuple(got)
     if any(t.device != tensors[0].device for t in tensors):
         raise ValueError("all tensors must be on one device")
-    norm = torch.stack([t.float().square().sum(dtype=torch.float64) for t in tensors]).sum().sqrt()
+    norm = torch.stack([t.double().square().sum() for t in tensors]).sum().sqrt()
     return norm.float(), (max_norm / (norm + eps)).clamp(max=1.0).float()
 
 

@@ -75,24 +75,32 @@ LAH_DEVINL void load8(const void* p, long i, float (&v)[8]) {
 
 LAH_DEVINL bool aligned16(const void* p) { return ((unsigned long long)p & 15) == 0; }
 
-template <int KIND>
-LAH_DEVINL float chunk_squares(const void* p, long from, long to) {
-  float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+// a thread's squares in a chunk, added in T
+template <int KIND, typename T>
+LAH_DEVINL T chunk_squares(const void* p, long from, long to) {
+  T s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (aligned16(p) && to - from == CLIP_CHUNK) {
 #pragma unroll
     for (int i = 0; i < CLIP_CHUNK / 2048; ++i) {
       float v[8];
       load8<KIND>(p, from + i * 2048 + threadIdx.x * 8, v);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) s[q] += v[q] * v[q];
+      for (int q = 0; q < 8; ++q) s[q] += (T)v[q] * (T)v[q];
     }
   } else {
     for (long i = from + threadIdx.x; i < to; i += 256) {
-      const float v = load_one<KIND>(p, i);
+      const T v = (T)load_one<KIND>(p, i);
       s[0] += v * v;
     }
   }
   return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+}
+
+// In fp32; where finite gradients of 2^64 and more leave its range, again in fp64.
+template <int KIND>
+LAH_DEVINL double squares_of(const void* p, long from, long to) {
+  const float s = chunk_squares<KIND, float>(p, from, to);
+  return isinf(s) ? chunk_squares<KIND, double>(p, from, to) : (double)s;
 }
 
 LAH_DEVINL double block_sum(double v, double* lds) {
@@ -112,9 +120,9 @@ __launch_bounds__(256) __global__ void clip_squares_kernel(ClipTensors a, double
   for (int c = blockIdx.x; c < a.first[a.count]; c += gridDim.x) {
     const int t = tensor_of(a, c);
     const long from = (long)(c - a.first[t]) * CLIP_CHUNK, to = min(from + CLIP_CHUNK, a.n[t]);
-    if (a.kind[t] == CLIP_F32) sum += chunk_squares<CLIP_F32>(a.p[t], from, to);
-    else if (a.kind[t] == CLIP_BF16) sum += chunk_squares<CLIP_BF16>(a.p[t], from, to);
-    else sum += chunk_squares<CLIP_F16>(a.p[t], from, to);
+    if (a.kind[t] == CLIP_F32) sum += squares_of<CLIP_F32>(a.p[t], from, to);
+    else if (a.kind[t] == CLIP_BF16) sum += squares_of<CLIP_BF16>(a.p[t], from, to);
+    else sum += squares_of<CLIP_F16>(a.p[t], from, to);
   }
   sum = block_sum(sum, lds);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;

@@ -180,3 +180,23 @@ def test_kernels_refuse_tangents():
                 _C.grouped_linear(args[0], args[1], off, args[2])
         with pytest.raises(NotImplementedError, match="forward-mode"):
             _C.ragged_nt(fwd.make_dual(x, x), w, off)
+
+
+@pytest.mark.parametrize("dtypes", [(torch.float32,), (torch.bfloat16,), (torch.float32, torch.bfloat16)], ids=str)
+def test_norm_of_large_gradients(dtypes):
+    """Finite gradients whose squares are beyond fp32 have a finite norm."""
+    g = torch.Generator(device="cpu").manual_seed(0)
+    ts = [torch.randn(n, device="cpu", generator=g).mul(s).to(dtypes[i % len(dtypes)]) for i, (n, s) in enumerate(
+        [(16384, 1e25), (5, 1e30), (100_003, 1.0), (40_000, 1e19)])]
+    want = torch.stack([t.double().square().sum() for t in ts]).sum().sqrt()
+    norm, scale = Fops.grad_clip_scale(ts, 2.0)
+    # squares and up to 64 sums in fp32, all positive: 2^-18 of the sum
+    assert torch.isfinite(norm) and (norm.double() - want).abs() <= 2.0 ** -18 * want
+    assert (scale.double() * want - 2.0).abs() <= 2 * 2.0 ** -18 * 2.0
+    mine = [t.clone() for t in ts]
+    Fops.clip_grad_norm_(mine, 2.0)
+    after = torch.stack([t.double().square().sum() for t in mine]).sum().sqrt()
+    # each element rounded to its type, and what was 1.0 is gone below fp32's range beside the largest
+    assert (after - 2.0).abs() <= 2 * max(torch.finfo(t).eps / 2 for t in dtypes) * 2.0 + 2.0 ** -16
+    ts[2][7] = float("inf")
+    assert torch.isinf(Fops.grad_clip_scale(ts, 2.0)[0]) and Fops.grad_clip_scale(ts, 2.0)[1] == 0
