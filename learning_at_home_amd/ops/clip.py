@@ -25,6 +25,13 @@ def _listed(tensors) -> list:
     return tensors
 
 
+def _check_distinct(tensors, name) -> None:
+    """Those that are written: on a GPU by many blocks at once."""
+    at = [t.data_ptr() for t in tensors if t.numel() and t.device.type != "meta"]
+    if len(set(at)) < len(at):
+        raise ValueError(f"the same tensor twice among the {name}")
+
+
 @torch.no_grad()
 def grad_clip_scale(tensors: Sequence[torch.Tensor], max_norm: float,
                     eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -49,8 +56,10 @@ def grad_clip_scale(tensors: Sequence[torch.Tensor], max_norm: float,
 def clip_grad_norm_(tensors: Sequence[torch.Tensor], max_norm: float,
                     eps: float = 1e-6) -> torch.Tensor:
     """Scales the tensors in place to a common 2-norm of at most max_norm, and
-    returns the norm they had, on their device."""
+    returns the norm they had, on their device. No tensor may be there twice."""
     tensors = _listed(tensors)
+    if not (HAS_HIP and tensors[0].is_cuda):  # where the kernels check the same
+        _check_distinct(tensors, "tensors")
     norm, scale = grad_clip_scale(tensors, max_norm, eps)
     if not (HAS_HIP and tensors[0].is_cuda and _C.grad_scale_(tensors, scale)):
         for t in tensors:
@@ -69,7 +78,8 @@ def master_sgd_step_(params: Sequence[torch.Tensor], masters: Sequence[torch.Ten
         u = grad_scale * g + weight_decay * m
         b = momentum * b + u, u = b          (with momentum_bufs)
         m -= lr * u;  p = m rounded to p's type
-    """
+
+    No parameter, master or buffer may be there twice."""
     params, masters, grads = list(params), list(masters), list(grads)
     bufs = list(momentum_bufs) if momentum_bufs is not None else []
     if not len(params) == len(masters) == len(grads) or (bufs and len(bufs) != len(params)):
@@ -88,6 +98,8 @@ def master_sgd_step_(params: Sequence[torch.Tensor], masters: Sequence[torch.Ten
             raise ValueError("params, masters and grads must have the same shapes")
         if any(p.shape != b.shape for p, b in zip(params, bufs)):
             raise ValueError("momentum_bufs must have the shapes of the params")
+        for name, ts in (("params", params), ("masters", masters), ("momentum_bufs", bufs)):
+            _check_distinct(ts, name)
     for i in range(len(params)):
         b = bufs[i : i + 1]
         if HAS_HIP and params[i].is_cuda and _C.master_sgd_(params[i : i + 1], masters[i : i + 1], grads[i : i + 1],

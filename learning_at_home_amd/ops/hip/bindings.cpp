@@ -5,6 +5,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 extern "C" {
 void lah_batched_gemm_nt(const void*, const void*, void*, const void*, void*, int, int,
                          int, int, int, hipStream_t);
@@ -770,6 +772,16 @@ struct ClipList {
   }
 };
 
+// One launch writes them all: a tensor that is there twice would be written by two blocks at once.
+static void check_distinct(const ClipList& l, const char* name) {
+  std::vector<void*> p;
+  p.reserve(l.p.size());
+  for (size_t i = 0; i < l.p.size(); ++i)
+    if (l.n[i] > 0) p.push_back(l.p[i]);
+  std::sort(p.begin(), p.end());
+  TORCH_CHECK_VALUE(std::adjacent_find(p.begin(), p.end()) == p.end(), "the same tensor twice among the ", name);
+}
+
 // (norm, scale); nothing where a tensor is not the kernels'
 std::vector<torch::Tensor> grad_norm(const std::vector<torch::Tensor>& grads, double max_norm, double eps) {
   const ClipList l(grads);
@@ -788,6 +800,7 @@ std::vector<torch::Tensor> grad_norm(const std::vector<torch::Tensor>& grads, do
 bool grad_scale_(const std::vector<torch::Tensor>& grads, const torch::Tensor& scale) {
   const ClipList l(grads);
   if (!l.taken) return false;
+  check_distinct(l, "tensors");
   const void* s = scale_ptr(scale, grads[0]);
   ON_DEVICE_OF(grads[0]);
   lah_grad_scale(l.p.data(), l.n.data(), l.kind.data(), (int)l.p.size(), s, cur_stream());
@@ -818,10 +831,13 @@ bool master_sgd_(const std::vector<torch::Tensor>& params, const std::vector<tor
   if (!bufs.empty()) {
     const ClipList l(bufs);
     taken = taken && l.taken && bufs[0].device() == params[0].device();
+    if (taken) check_distinct(l, "momentum_bufs");
     b = l.p;
   }
   for (const int k : p.kind) taken = taken && k == 0;
   if (!taken) return false;
+  check_distinct(p, "params");
+  check_distinct(m, "masters");
   const void* s = scale_ptr(scale, params[0]);
   ON_DEVICE_OF(params[0]);
   lah_master_sgd(p.p.data(), m.p.data(), g.p.data(), b.empty() ? nullptr : b.data(), p.n.data(),

@@ -276,3 +276,20 @@ def test_norm_of_large_gradients(dtypes):
     assert (after - 2.0).abs() <= 2 * max(torch.finfo(t).eps / 2 for t in dtypes) * 2.0 + 2.0 ** -16
     ts[2][7] = float("inf")
     assert torch.isinf(Fops.grad_clip_scale(ts, 2.0)[0]) and Fops.grad_clip_scale(ts, 2.0)[1] == 0
+
+
+def test_the_same_tensor_twice():
+    """Written twice at once it would be scaled or stepped once or twice: refused, and nothing is written."""
+    a, b = torch.ones(5, device=DEV), torch.ones(5, device=DEV)
+    with pytest.raises(ValueError, match="twice"):
+        Fops.clip_grad_norm_([a, b, a], 0.5)
+    p, m, v = ([torch.ones(5, device=DEV).to(t) for _ in range(2)] for t in (torch.bfloat16, torch.float32, torch.float32))
+    for change in (dict(params=[p[0], p[0]]), dict(masters=[m[0], m[0]]), dict(momentum_bufs=[v[1], v[1]])):
+        args = dict(params=p, masters=m, grads=[a, a], lr=0.1, momentum=0.9, momentum_bufs=v)
+        with pytest.raises(ValueError, match="twice"):
+            Fops.master_sgd_step_(**{**args, **change})
+    assert all((t == 1).all() for t in (a, b, *p, *m, *v))
+    empty = torch.ones(0, device=DEV)
+    Fops.clip_grad_norm_([empty, a, empty], 0.5)
+    Fops.master_sgd_step_(p, m, [b, b], lr=0.1)  # read twice is fine
+    assert (m[0] == m[1]).all() and (m[0] < 1).all()
