@@ -88,6 +88,10 @@ def master_sgd_step_(params: Sequence[torch.Tensor], masters: Sequence[torch.Ten
         raise ValueError("momentum needs momentum_bufs")
     if not params:
         return
+    if isinstance(grad_scale, torch.Tensor) and (grad_scale.numel() != 1 or (
+            params[0].is_cuda and grad_scale.device != params[0].device)):
+        raise ValueError(f"grad_scale must be one number on the params' device, got {tuple(grad_scale.shape)} "
+                         f"on {grad_scale.device}")
     if HAS_HIP and params[0].is_cuda:  # with the same checks
         if _C.master_sgd_(params, masters, grads, bufs, grad_scale, lr, momentum, weight_decay):
             return

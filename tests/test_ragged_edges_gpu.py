@@ -293,3 +293,16 @@ def test_the_same_tensor_twice():
     Fops.clip_grad_norm_([empty, a, empty], 0.5)
     Fops.master_sgd_step_(p, m, [b, b], lr=0.1)  # read twice is fine
     assert (m[0] == m[1]).all() and (m[0] < 1).all()
+
+
+def test_scale_is_one_number():
+    """A vector as long as a tensor would scale it element by element on the CPU."""
+    p, m, g = (torch.ones(3, device=DEV) for _ in range(3))
+    for scale in (torch.ones(3, device=DEV), torch.ones(0, device=DEV)):
+        with pytest.raises(ValueError, match="one number"):
+            Fops.master_sgd_step_([p], [m], [g], lr=0.1, grad_scale=scale)
+    with pytest.raises(ValueError, match="one number"):
+        Fops.master_sgd_step_([p], [m], [g], lr=0.1, grad_scale=torch.ones(()))
+    assert (m == 1).all()
+    Fops.master_sgd_step_([p], [m], [g], lr=0.5, grad_scale=torch.full((1,), 0.5, device=DEV))
+    assert (m == 0.75).all()
