@@ -23,7 +23,7 @@ from learning_at_home_amd.models import TransformerDMoE, TransformerDMoEConfig
 from learning_at_home_amd.parallel import ExpertParallelMoE, FusedExpertSGD
 from learning_at_home_amd.averaging import RcclAverager
 from learning_at_home_amd.ops import HAS_HIP
-from learning_at_home_amd.ops.functional import grad_clip_scale
+from learning_at_home_amd.ops.functional import clip_grad_norm_, grad_clip_scale
 from learning_at_home_amd.optim import MasterSGD
 
 
@@ -236,6 +236,8 @@ def main():
         if args.clip_norm > 0 and use_cuda:
             grads = trunk_opt.gradients() + [g for opt in expert_opts for g in opt.gradients()]
             scale = grad_clip_scale(grads, args.clip_norm)[1]
+        elif args.clip_norm > 0:  # plain optimizers take no scale: the gradients themselves
+            clip_grad_norm_([p.grad for p in model.parameters() if p.grad is not None], args.clip_norm)
         scaled = {} if scale is None else {"grad_scale": scale}
         with tm("expert_opt"):
             for opt in expert_opts:
@@ -327,7 +329,8 @@ def main():
                 "global_batch": B * world_size,
                 "seq_len": cfg.seq_len,
                 "parallelism": par,
-                "capacity_factor": args.capacity_factor,
+                "capacity_factor": None if args.dropless else args.capacity_factor,
+                **({"clip_norm": args.clip_norm} if args.clip_norm > 0 else {}),
                 "dropped_token_frac": dropped_frac,
                 "last_loss": round(float(last_loss), 4) if last_loss is not None else None,
             },

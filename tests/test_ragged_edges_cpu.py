@@ -1,7 +1,9 @@
 """Calls at the edges of the ragged expert path, on the CPU: arguments that do not go
 together, no tokens, weights of little mass, derivatives that the operators do not have."""
+import json
 import os
 import socket
+import sys
 
 import pytest
 import torch
@@ -228,3 +230,28 @@ def test_scale_is_one_number():
     assert (m == 1).all()
     Fops.master_sgd_step_([p], [m], [g], lr=0.5, grad_scale=torch.full((1,), 0.5))
     assert (m == 0.75).all()
+
+
+def test_bench_says_what_it_ran(monkeypatch, capsys):
+    """A line without capacity, or with clipped steps, does not read as the default's; and the CPU clips."""
+    import bench
+
+    clipped = []
+
+    def record(grads, max_norm):
+        before = Fops.clip_grad_norm_(grads, max_norm)
+        clipped.append((len(grads), float(before), float(Fops.grad_clip_scale(grads, max_norm)[0])))
+        return before
+
+    monkeypatch.setattr(bench, "clip_grad_norm_", record)
+    got = []
+    for flags in ([], ["--dropless", "--clip-norm", "0.001"]):
+        monkeypatch.setattr(sys, "argv", ["bench.py", "--steps", "2", "--warmup", "0", "--no-dht", *flags])
+        bench.main()
+        got.append(json.loads(capsys.readouterr().out.strip().splitlines()[-1])["config"])
+        assert bool(clipped) == bool(flags)
+    assert got[0]["capacity_factor"] == 1.5 and "clip_norm" not in got[0]
+    assert got[1]["capacity_factor"] is None and got[1]["clip_norm"] == 0.001
+    assert len(clipped) == 2
+    for count, before, after in clipped:
+        assert count > 8 and before > 0.001 and abs(after - 0.001) < 1e-6
