@@ -1,6 +1,7 @@
 """Calls at the edges of the ragged expert path, on the CPU: arguments that do not go
 together, no tokens, weights of little mass, derivatives that the operators do not have."""
 import json
+import multiprocessing
 import os
 import socket
 import sys
@@ -244,6 +245,7 @@ def test_bench_says_what_it_ran(monkeypatch, capsys):
         return before
 
     monkeypatch.setattr(bench, "clip_grad_norm_", record)
+    monkeypatch.setattr(multiprocessing, "set_start_method", lambda *a, **k: None)  # the tests' own stays
     got = []
     for flags in ([], ["--dropless", "--clip-norm", "0.001"]):
         monkeypatch.setattr(sys, "argv", ["bench.py", "--steps", "2", "--warmup", "0", "--no-dht", *flags])
