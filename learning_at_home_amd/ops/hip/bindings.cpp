@@ -511,8 +511,9 @@ std::vector<torch::Tensor> ragged_layout(torch::Tensor ids, int64_t E) {
 // Tiles of 256 x 256 (one block a CU, a list of tiles) or 128 x 256: the large ones where
 // there are some for half the CUs and experts have rows for them. Large against small, us:
 // 8 experts of 512 rows, 1024 -> 1024 (64 tiles) 29 and 25, of 1024 rows (128) 31 and 38;
-// 256 experts, 1024 -> 4096, of 32 rows 405 and 452, of 64 rows 422 and 508; 4096 -> 1024, of
-// 64 rows 537 and 458, of 96 rows 522 and 550, of 256 rows 633 and 1071.
+// 256 experts, 1024 -> 4096, of 64 rows 422 and 508; 4096 -> 1024, of 64 rows 537 and 458, of
+// 96 rows 522 and 550, of 256 rows 633 and 1071. At 32 rows neither has all: 1024 -> 4096, even
+// rows 383 and 419, uneven ones with gelu 459 and 435; 4096 -> 1024, 470 and 380.
 static bool large_tiles(int64_t R, int64_t E, int64_t N) {
   const int64_t tiles = R / 256 * ((N + 255) / 256);
   return (R >= 96 * E && tiles >= 128) || (R >= 64 * E && tiles >= 512);
