@@ -231,11 +231,15 @@ std::vector<torch::Tensor> assign_slots(torch::Tensor topk_idx, int64_t E, int64
   return {pos, counts, inv};
 }
 
+// dispatch.hip has a wave for each row, and a launch below 2^32 threads
+#define CHECK_WAVES(rows) TORCH_CHECK((rows) < (int64_t)1 << 26, "below 2^26 rows, got ", rows)
+
 // What a kernel of dispatch.hip takes rows and slots from: [T, k] int32, on the rows' GPU
 static void check_slots(const torch::Tensor& rows, const torch::Tensor& topk_idx, const torch::Tensor& pos) {
   CHECK_CUDA(rows);
   CHECK_I32(topk_idx); CHECK_I32(pos);
   TORCH_CHECK(topk_idx.dim() == 2 && topk_idx.sizes() == pos.sizes(), "topk_idx and pos must be [T, k]");
+  CHECK_WAVES(topk_idx.size(0));
   TORCH_CHECK(topk_idx.device() == rows.device() && pos.device() == rows.device(),
               "all tensors must be on one GPU");
 }
@@ -243,6 +247,7 @@ static void check_slots(const torch::Tensor& rows, const torch::Tensor& topk_idx
 static void check_buffer(const torch::Tensor& buf) {
   CHECK_BF16(buf);
   TORCH_CHECK(buf.dim() == 3, "the buffer must be [E, C, D]");
+  CHECK_WAVES(buf.size(0) * buf.size(1));
   TORCH_CHECK(buf.size(2) % 8 == 0, "D must be a multiple of 8");
 }
 
@@ -253,6 +258,7 @@ torch::Tensor dispatch_gather(torch::Tensor x, torch::Tensor inv, int64_t k) {
   int E = inv.size(0), C = inv.size(1), D = x.size(1);
   TORCH_CHECK(D % 8 == 0, "D must be a multiple of 8");
   TORCH_CHECK(k > 0 || inv.numel() == 0, "k must be positive");
+  CHECK_WAVES(inv.numel());
   ON_DEVICE_OF(x);
   x = ready(x);
   inv = inv.contiguous();

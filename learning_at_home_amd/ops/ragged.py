@@ -121,16 +121,18 @@ def _check_layout(layout, t, name):
         raise ValueError(f"{name} and the layout must be on one device")
 
 
-def _check_gpu_rows(t, name):
+def _check_gpu_rows(t, name, rows=0):
     if t.dtype != torch.bfloat16:
         raise ValueError(f"the GPU kernels take bf16, got {name} in {t.dtype}")
     if t.shape[1] % 8:
         raise ValueError(f"{name} must have a multiple of 8 columns (16-byte rows), got {tuple(t.shape)}")
+    if max(t.shape[0], rows) >= 1 << 26:  # a wave each, and 2^32 threads a launch
+        raise ValueError(f"below 2^26 tokens and rows, got {t.shape[0]} and {rows}")
 
 
 def ragged_gather(x: torch.Tensor, layout: RaggedLayout) -> torch.Tensor:
     """x [T, D] -> the layout's rows [T * k, D]; rows of nobody are zeros. On a
-    GPU: bf16, D a multiple of 8."""
+    GPU: bf16, D a multiple of 8, below 2^26 rows."""
     from .functional import dispatch
 
     _check_layout(layout, x, "x")
@@ -138,7 +140,7 @@ def ragged_gather(x: torch.Tensor, layout: RaggedLayout) -> torch.Tensor:
     if x.dim() != 2 or x.shape[0] != T:
         raise ValueError(f"x must be [{T}, D], a row for each token of the layout, got {tuple(x.shape)}")
     if x.is_cuda and HAS_HIP:
-        _check_gpu_rows(x, "x")
+        _check_gpu_rows(x, "x", layout.order.numel())
         return _GatherHip.apply(_ready(x), layout.rows, layout.order)
     one = torch.zeros_like(layout.rows)  # all rows in one group: their number is their slot
     return dispatch(x, one, layout.rows, layout.order.unsqueeze(0), k)[0]
@@ -159,7 +161,7 @@ def ragged_combine(y: torch.Tensor, layout: RaggedLayout, weights: torch.Tensor,
     normalised over the slots that have a row: divided by their sum, or by
     min_mass where that is larger (the bound on 1 / sum that functional.combine
     has behind a capacity, 0.2). A sum of zero or less gives zeros. On a GPU: y
-    bf16, D a multiple of 8, weights fp32."""
+    bf16, D a multiple of 8, weights fp32, below 2^26 rows."""
     from .functional import combine
 
     if not min_mass >= 0:

@@ -64,7 +64,8 @@ class TestRowsRefuse:
             Fops.ragged_ungather(y, self.layout)
 
     @pytest.mark.parametrize("t,match", [(torch.zeros(3, 8), "bf16"), (torch.zeros(3, 8).half(), "bf16"),
-                                         (torch.zeros(3, 12).bfloat16(), "multiple of 8")])
+                                         (torch.zeros(3, 12).bfloat16(), "multiple of 8"),
+                                         (torch.empty(1 << 26, 8, device="meta", dtype=torch.bfloat16), "2.26")])
     def test_what_the_kernels_do_not_take(self, t, match):
         with pytest.raises(ValueError, match=match):
             ragged._check_gpu_rows(t, "x")
