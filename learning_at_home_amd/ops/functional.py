@@ -160,11 +160,12 @@ class _Combine(torch.autograd.Function):
 
 def _survivor_weights(pos, w, min_mass=0.2):
     surv = pos >= 0
-    s = (w * surv).sum(-1, keepdim=True)
+    w = w.masked_fill(~surv, 0)  # whatever a dropped slot's weight is
+    s = w.sum(-1, keepdim=True)
     # clamped renormalization (matches dispatch.hip): bounds the gradient
     # amplification when capacity drops remove most of the softmax mass
     inv_s = torch.where(s > 0, 1.0 / s.clamp(min=min_mass), torch.zeros_like(s))
-    return (w * surv) * inv_s, surv, inv_s
+    return w * inv_s, surv, inv_s
 
 
 def _combine_fwd_torch(ybuf, topk_idx, pos, w, min_mass=0.2):
@@ -172,8 +173,8 @@ def _combine_fwd_torch(ybuf, topk_idx, pos, w, min_mass=0.2):
     T, k = topk_idx.shape
     w_hat, surv, _ = _survivor_weights(pos, w, min_mass)
     flat = (topk_idx.long() * C + pos.clamp(min=0).long()).view(-1)
-    rows = ybuf.view(-1, D)[flat].view(T, k, D)
-    return (w_hat.unsqueeze(-1).to(rows.dtype) * rows * surv.unsqueeze(-1)).sum(1)
+    rows = ybuf.view(-1, D)[flat].view(T, k, D).masked_fill(~surv.unsqueeze(-1), 0)
+    return (w_hat.unsqueeze(-1).to(rows.dtype) * rows).sum(1)
 
 
 def _combine_bwd_torch(dy, ybuf, y, topk_idx, pos, w, min_mass=0.2):
@@ -189,9 +190,9 @@ def _combine_bwd_torch(dy, ybuf, y, topk_idx, pos, w, min_mass=0.2):
     rows = ybuf.view(-1, D)[(topk_idx.long() * C + pos.clamp(min=0).long()).view(-1)].view(T, k, D)
     dot_yj = torch.einsum("td,tkd->tk", dy.float(), rows.float())
     dot_y = torch.einsum("td,td->t", dy.float(), y.float()).unsqueeze(-1)
-    s = (w * surv).sum(-1, keepdim=True)
+    s = w.masked_fill(~surv, 0).sum(-1, keepdim=True)
     clamped = (s > 0) & (s < min_mass)  # in the clamp region d(w/min_mass)/dw is diagonal
-    dw = (torch.where(clamped, dot_yj, dot_yj - dot_y) * inv_s) * surv
+    dw = (torch.where(clamped, dot_yj, dot_yj - dot_y) * inv_s).masked_fill(~surv, 0)
     return dybuf, dw.float()
 
 

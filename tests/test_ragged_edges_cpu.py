@@ -258,3 +258,31 @@ def test_bench_says_what_it_ran(monkeypatch, capsys):
     assert len(clipped) == 2
     for count, before, after in clipped:
         assert count > 8 and before > 0.001 and abs(after - 0.001) < 1e-6
+
+
+def test_masked_slots_reach_nothing():
+    """NaN and infinity in a masked slot's weight, in rows of nobody or in another token's row stay there."""
+    g = torch.Generator().manual_seed(0)
+    ids = torch.tensor([[2, 0], [-1, 1], [1, -1], [-1, -1], [0, 2]], dtype=torch.int32).to("cpu")
+    layout = Fops.ragged_layout(ids, 3)
+    y = torch.randn(10, 8, generator=g).to("cpu", torch.float32)
+    w, dy = torch.rand(5, 2, generator=g).to("cpu"), torch.randn(5, 8, generator=g).to("cpu", torch.float32)
+
+    def run(y, w):
+        y, w = y.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        out = Fops.ragged_combine(y, layout, w)
+        return (out.detach(), *torch.autograd.grad(out, (y, w), dy))
+
+    clean = run(y, w)
+    y2, w2 = y.clone(), w.clone()
+    y2[6:] = float("nan")  # rows of nobody
+    w2[1, 0], w2[2, 1], w2[3, 0] = float("nan"), float("inf"), float("nan")
+    for a, b in zip(run(y2, w2), clean):
+        assert torch.equal(a, b)
+    y2[0] = float("inf")  # row 0 is token 0's or 4's, which alone may see it
+    token = int((layout.rows == 0).any(1).nonzero())
+    keep = [t for t in range(5) if t != token]
+    out, dyy, dw = run(y2, w2)
+    assert torch.equal(out[keep], clean[0][keep]) and torch.equal(dw[keep], clean[2][keep])
+    own = layout.rows[token].tolist()
+    assert all(torch.equal(dyy[r], clean[1][r]) for r in range(10) if r not in own)
