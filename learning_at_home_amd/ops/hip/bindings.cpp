@@ -645,7 +645,7 @@ torch::Tensor ragged_slope(torch::Tensor dy, torch::Tensor der, torch::Tensor of
               dy.size(1) < 1 << 21, "dy and der must be [R, N], N a multiple of 8");
   TORCH_CHECK(write || db.has_value(), "nothing is asked for");
   const int64_t R = dy.size(0), N = dy.size(1), E = offsets.numel() - 1;
-  TORCH_CHECK(E <= 65535, "too many groups");
+  TORCH_CHECK(E <= 4096, "at most 4096 groups, got ", E);
   void* db_p = nullptr;
   int db_bf16 = 0;
   if (db.has_value()) {

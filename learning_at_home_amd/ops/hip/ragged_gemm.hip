@@ -1566,86 +1566,112 @@ extern "C" void lah_ragged_tn(const void* d, const void* x, void* dw, void* db, 
   else launch_weights<R_F32>(a, table, stream);
 }
 
+// The group of a slot (find_expert) in two steps of 64: starts grow with the group. Each block
+// of the pass below looks for its own, and many have few rows: 4096 groups of 2048 rows, 4096
+// columns, 52 us, 345 with find_expert's 65 ballots.
+LAH_DEVINL int find_slot(const int* __restrict__ offsets, int E, int slot) {
+  const int lane = threadIdx.x & 63;
+  auto begun = [&](int e) { return e < E && (e > 0 ? offsets[e] : 0) / RBM + e <= slot; };
+  const int base = (__popcll(__ballot(begun(lane * 64))) - 1) * 64;
+  const int e = base + __popcll(__ballot(begun(base + lane))) - 1;
+  return offsets[E] / RBM + E <= slot ? E : e;  // rows of nobody
+}
+
 // dP = dy * slope, rounded to bf16 for the two products that take it, and db, its sums over each
-// group's rows as they were before that. A block has up to 128 rows of one group by 256
-// columns, 8 a lane; where there are fewer columns its lanes take more rows. Its sums go to
-// part[slot], and are joined in the slots' order. Or it has a whole group, by 64 columns, and
-// needs no join. Rows of nobody are left out: nothing reads their dP. Bound by HBM: dy and the
-// slope in, dP out. 262144 rows of 4096: 1236 us, 6.4 GB at 5.2 TB/s, and 1217 without db.
+// group's rows as they were before that. A tile is up to 128 rows of one group by 256 columns,
+// 8 a lane; where there are fewer columns its lanes take more rows. Its sums go to part[slot],
+// and are joined in the slots' order. Or it is a whole group, by 64 columns, and needs no join.
+// Rows of nobody are left out: nothing reads their dP. Bound by HBM: dy and the slope in, dP out.
+// 262144 rows of 4096: 1236 us, 6.4 GB at 5.2 TB/s, and 1217 without db.
 enum { S_NONE = 0, S_PART = 1, S_GROUP = 2 };  // sums: none, of a tile, of a group
 template <bool WRITE, int SUMS>
 __launch_bounds__(256) __global__ void ragged_slope_kernel(RaggedArgs a, const __bf16* __restrict__ dy,
                                                            __bf16* __restrict__ dp, float* __restrict__ part,
-                                                           int shift) {
+                                                           int shift, int tiles) {
   __shared__ __attribute__((aligned(16))) float sums[2048];  // [row lanes][columns]
-  const int lanes = 1 << shift, NT = cdiv(a.N, lanes * 8), L = blockIdx.y * gridDim.x + blockIdx.x, slot = L / NT;
-  const int e = SUMS == S_GROUP ? slot : __builtin_amdgcn_readfirstlane(find_expert<RBM>(a.offsets, a.E, slot));
-  long lo, hi;
-  expert_rows(a, e, &lo, &hi);
-  const long row0 = SUMS == S_GROUP ? lo : lo + (long)(slot - (int)(lo / RBM) - e) * RBM;
-  if (e >= a.E || (SUMS != S_GROUP && (row0 < lo || row0 >= hi))) return;
-  const int rows = (int)(SUMS == S_GROUP ? hi - lo : min(hi - row0, (long)RBM)), c = threadIdx.x & (lanes - 1), r0 = threadIdx.x >> shift;
-  const int n0 = L % NT * lanes * 8, n = n0 + c * 8, step = 256 >> shift;
-  float sum[8] = {};
-  if (n < a.N) {
-    const long at = row0 * a.N + n;
-    for (int r = r0; r < rows; r += 4 * step) {  // four rows' loads at once
-      bf16x8 y[4];
-      f16x8 d[4];
+  const int lanes = 1 << shift, NT = cdiv(a.N, lanes * 8), step = 256 >> shift;
+  const int c = threadIdx.x & (lanes - 1), r0 = threadIdx.x >> shift;
+  for (int L = blockIdx.x; L < tiles; L += gridDim.x) {
+    const int slot = L / NT, n0 = L % NT * lanes * 8, n = n0 + c * 8;
+    const int e = SUMS == S_GROUP ? slot : __builtin_amdgcn_readfirstlane(find_slot(a.offsets, a.E, slot));
+    if (e < 0 || e >= a.E) continue;
+    long lo, hi;
+    expert_rows(a, e, &lo, &hi);
+    const long row0 = SUMS == S_GROUP ? lo : lo + (long)(slot - (int)(lo / RBM) - e) * RBM;
+    if (SUMS != S_GROUP && (row0 < lo || row0 >= hi)) continue;
+    const int rows = (int)(SUMS == S_GROUP ? hi - lo : min(hi - row0, (long)RBM));
+    float sum[8] = {};
+    if (n < a.N) {
+      const long at = row0 * a.N + n;
+      for (int r = r0; r < rows; r += 4 * step) {  // four rows' loads at once
+        bf16x8 y[4];
+        f16x8 d[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const bool in = r + u * step < rows;
-        y[u] = in ? *(const bf16x8*)(dy + at + (long)(r + u * step) * a.N) : bf16x8{};
-        d[u] = in ? *(const f16x8*)(a.der + at + (long)(r + u * step) * a.N) : f16x8{};
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        bf16x8 o;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const float v = bf2f(y[u][x]) * (float)d[u][x];
-          sum[x] += v;
-          o[x] = f2bf(v);
+        for (int u = 0; u < 4; ++u) {
+          const bool in = r + u * step < rows;
+          y[u] = in ? *(const bf16x8*)(dy + at + (long)(r + u * step) * a.N) : bf16x8{};
+          d[u] = in ? *(const f16x8*)(a.der + at + (long)(r + u * step) * a.N) : f16x8{};
         }
-        if (WRITE && r + u * step < rows) *(bf16x8*)(dp + at + (long)(r + u * step) * a.N) = o;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          bf16x8 o;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float v = bf2f(y[u][x]) * (float)d[u][x];
+            sum[x] += v;
+            o[x] = f2bf(v);
+          }
+          if (WRITE && r + u * step < rows) *(bf16x8*)(dp + at + (long)(r + u * step) * a.N) = o;
+        }
       }
     }
-  }
-  if (SUMS == S_NONE) return;
+    if (SUMS == S_NONE) continue;
 #pragma unroll
-  for (int h = 0; h < 8; h += 4)
-    *(f32x4*)(sums + (r0 * lanes + c) * 8 + h) = f32x4{sum[h], sum[h + 1], sum[h + 2], sum[h + 3]};
-  __syncthreads();
-  const int col = threadIdx.x;
-  if (col >= lanes * 8 || n0 + col >= a.N) return;
-  float all = 0.f;
-  for (int r = 0; r < step; ++r) all += sums[r * lanes * 8 + col];
-  const long to = (long)slot * a.N + n0 + col;
-  if (SUMS == S_PART) part[to] = all;
-  else if (a.bias_bf16) ((__bf16*)a.db)[to] = f2bf(all);
-  else ((float*)a.db)[to] = all;
+    for (int h = 0; h < 8; h += 4)
+      *(f32x4*)(sums + (r0 * lanes + c) * 8 + h) = f32x4{sum[h], sum[h + 1], sum[h + 2], sum[h + 3]};
+    __syncthreads();
+    const int col = threadIdx.x;
+    if (col < lanes * 8 && n0 + col < a.N) {
+      float all = 0.f;
+      for (int r = 0; r < min(step, rows); ++r) all += sums[r * lanes * 8 + col];  // lanes past the rows have none
+      const long to = (long)slot * a.N + n0 + col;
+      if (SUMS == S_PART) part[to] = all;
+      else if (a.bias_bf16) ((__bf16*)a.db)[to] = f2bf(all);
+      else ((float*)a.db)[to] = all;
+    }
+    __syncthreads();  // the next tile's sums
+  }
 }
 
-// db of each group from its slots' sums: four quarters of the slots in turn, joined in order
-__launch_bounds__(256) __global__ void ragged_join_sums_kernel(RaggedArgs a, const float* __restrict__ part) {
-  __shared__ float sums[4][64];
-  const int e = blockIdx.y, c = threadIdx.x & 63, q = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
-  long lo, hi;
-  expert_rows(a, e, &lo, &hi);
-  const int count = (int)((hi - lo + RBM - 1) / RBM);
-  float sum = 0.f;
-  if (n < a.N) {
-    const float* at = part + ((lo / RBM) + e) * a.N + n;
+// db of each group from its slots' sums, four columns a lane: four quarters of the slots in turn,
+// joined in order
+__launch_bounds__(256) __global__ void ragged_join_sums_kernel(RaggedArgs a, const float* __restrict__ part, int tiles) {
+  __shared__ f32x4 sums[4][64];
+  const int c = threadIdx.x & 63, q = threadIdx.x >> 6, NT = cdiv(a.N, 256);
+  for (int L = blockIdx.x; L < tiles; L += gridDim.x) {
+    const int e = L / NT, n = L % NT * 256 + c * 4;
+    long lo, hi;
+    expert_rows(a, e, &lo, &hi);
+    const int count = (int)((hi - lo + RBM - 1) / RBM);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (n < a.N) {
+      const float* at = part + ((lo / RBM) + e) * a.N + n;
 #pragma unroll 8
-    for (int i = q; i < count; i += 4) sum += at[(long)i * a.N];
+      for (int i = q; i < count; i += 4) sum += *(const f32x4*)(at + (long)i * a.N);
+    }
+    sums[q][c] = sum;
+    __syncthreads();
+    if (q == 0 && n < a.N) {
+      const f32x4 all = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+      const long to = (long)e * a.N + n;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (a.bias_bf16) ((__bf16*)a.db)[to + x] = f2bf(all[x]);
+        else ((float*)a.db)[to + x] = all[x];
+      }
+    }
+    __syncthreads();
   }
-  sums[q][c] = sum;
-  __syncthreads();
-  if (q > 0 || n >= a.N) return;
-  const float all = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
-  const long to = (long)e * a.N + n;
-  if (a.bias_bf16) ((__bf16*)a.db)[to] = f2bf(all);
-  else ((float*)a.db)[to] = all;
 }
 
 // Whole groups where none can be long: 128 rows are a round of a block, and one more launch is
@@ -1665,13 +1691,18 @@ extern "C" void lah_ragged_slope(const void* dy, const void* der, void* dp, void
   const bool by_group = db != nullptr && slope_by_group(R);
   int shift = 0;
   while (shift < (by_group ? 3 : 5) && (8 << shift) < N) ++shift;
-  const long tiles = by_group ? E : R / RBM + E + 1, blocks = tiles * cdiv(N, 8 << shift);
-  const unsigned wide = (unsigned)(blocks < 1 << 22 ? blocks : 1 << 22);  // 2^32 threads a dimension
+  // many groups of few rows: more columns a tile
+  while (by_group && shift < 5 && (8 << shift) < N && (long)E * cdiv(N, 8 << shift) > 16384) ++shift;
+  const long tiles = (by_group ? E : R / RBM + E + 1) * cdiv(N, 8 << shift);
+  auto blocks = [](long n) { return dim3((unsigned)(n < 16384 ? n : 16384)); };
   auto kernel = dp == nullptr ? (by_group ? ragged_slope_kernel<false, S_GROUP> : ragged_slope_kernel<false, S_PART>)
                 : db == nullptr ? ragged_slope_kernel<true, S_NONE>
                 : by_group ? ragged_slope_kernel<true, S_GROUP> : ragged_slope_kernel<true, S_PART>;
-  hipLaunchKernelGGL(kernel, dim3(wide, (unsigned)((blocks + wide - 1) / wide)), dim3(256), 0, stream, a,
-                     (const __bf16*)dy, (__bf16*)dp, (float*)work, shift);
-  if (db != nullptr && !by_group)
-    hipLaunchKernelGGL(ragged_join_sums_kernel, dim3(cdiv(N, 64), E), dim3(256), 0, stream, a, (const float*)work);
+  hipLaunchKernelGGL(kernel, blocks(tiles), dim3(256), 0, stream, a, (const __bf16*)dy, (__bf16*)dp, (float*)work,
+                     shift, (int)tiles);
+  if (db != nullptr && !by_group) {
+    const long joined = (long)E * cdiv(N, 256);
+    hipLaunchKernelGGL(ragged_join_sums_kernel, blocks(joined), dim3(256), 0, stream, a, (const float*)work,
+                       (int)joined);
+  }
 }
